@@ -463,6 +463,101 @@ int qw_moe_route_backward(const float* probs, const int32_t* top_idx, const floa
                           const float* grad_probs, const float* grad_balance, const int32_t* counts, int64_t tokens,
                           int64_t experts, int64_t top_k, float temperature, float* grad_scores, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Routing by scores (layers with many experts).  No reference counterpart
+ * beyond the plain softmax top-k of src/quantweave_moe_model.py:124-137.
+ * ------------------------------------------------------------------------ */
+
+/* From fp32 logits [tokens, experts] (already divided by the temperature):
+ *   scores = softmax(logits) (score 0) or sigmoid(logits) (score 1)   [T, E]
+ *   choice = scores + bias        (bias NULL: scores)
+ *   of the `groups` equal runs of experts the top_groups of highest value stay,
+ *   a run's value being the sum of its group_top (1 or 2) highest choices
+ *   top_idx = the top_k highest choices among them, descending       [T, k]
+ *   top_w  = scores[top_idx] / (their sum + 1e-20) * scale, or without the
+ *            division when renormalize == 0                          [T, k]
+ *   probs  = scores / sum(scores) (NULL: not wanted; all 0 without a sum)
+ * The choice is that of 64-bit arithmetic on the logits; equal values go to the
+ * lowest index, a NaN counts as -infinity.  A softmax row of -infinities has
+ * scores 0.  1 <= experts <= 1024, groups divides experts, top_k <= 64 and at
+ * most the experts of top_groups groups. */
+int qw_moe_route_scored_from_logits(const float* logits, int64_t tokens, int64_t experts, int64_t top_k, int score,
+                                    const float* bias, int64_t groups, int64_t top_groups, int group_top,
+                                    int renormalize, float scale, float* scores, float* probs, int32_t* top_idx,
+                                    float* top_w, void* stream);
+
+/* The same behind the router's product: logits = x @ router_w^T / temperature,
+ * as qw_moe_route forms and stores them (its workspace). */
+int qw_moe_route_scored(const void* x, int x_dtype, int64_t x_row_stride, const void* router_w, int w_dtype,
+                        int64_t tokens, int64_t d_model, int64_t experts, int64_t top_k, float temperature, int score,
+                        const float* bias, int64_t groups, int64_t top_groups, int group_top, int renormalize,
+                        float scale, float* logits, float* scores, float* probs, int32_t* top_idx, float* top_w,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradient with respect to logits * temperature: from the gradients of
+ * top_w (NULL = 0), scores (NULL = 0), probs (NULL = 0) and of the balance loss
+ * over probs (grad_balance, a device scalar, NULL = 0; needs the plan's counts).
+ * The bias and the choice get none.  Indices outside the experts are skipped. */
+int qw_moe_route_scored_backward(const float* scores, const int32_t* top_idx, const float* grad_top_w,
+                                 const float* grad_scores, const float* grad_probs, const float* grad_balance,
+                                 const int32_t* counts, int64_t tokens, int64_t experts, int64_t top_k, int score,
+                                 int renormalize, float scale, float temperature, float* grad_logits, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Microscaled 4-bit floating point.  No reference counterpart (its 4-bit
+ * weights are integers, src/quantization.py:21-75).
+ *
+ * A row is blocks of 32 columns: codes of 4 bits (sign, two exponent bits, one
+ * mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two per byte with the even column
+ * in the low nibble, and one scale byte s per block, 2^(s - 127) (255: NaN).
+ * Columns are padded to whole 128 with zero codes: codes [rows, padded / 2],
+ * 16-byte aligned, scales [rows, padded / 32], 4-byte aligned.  Padding has to
+ * be zero codes under scales other than 255.
+ * ------------------------------------------------------------------------ */
+
+/* x [rows, cols] (row stride x_row_stride elements) -> codes and scales.  Per
+ * block the scale is 2^(floor(log2 max|x|) - 2), at least 2^-127; x / scale is
+ * rounded to the nearest code, ties to the even one, saturating at 6.  A block
+ * holding an infinity or a NaN gets scale 255 and zero codes. */
+int qw_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_row_stride, void* codes,
+                   void* scales, void* stream);
+
+/* codes and scales -> out [rows, cols] (contiguous), code * scale rounded once. */
+int qw_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int out_dtype,
+                     void* stream);
+
+/* out [rows, out_features] = x quantised as above, times the stored matrix
+ * [out_features, in_features] transposed: exact products summed in fp32 and
+ * rounded once to act_dtype (QW_F32, QW_BF16 or QW_F16, of x and out). */
+size_t qw_mx_matmul_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features);
+int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t rows, const void* codes,
+                 const void* scales, int64_t out_features, int64_t in_features, void* out, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/* grad_x [rows, in_features] = grad_out [rows, out_features] @ W, the stored
+ * matrix rounded to dtype first (exact for bf16 and fp32): the gradient of
+ * qw_mx_matmul with the quantisation of x passed over. */
+size_t qw_mx_matmul_backward_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features, int dtype);
+int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const void* codes, const void* scales,
+                          int64_t out_features, int64_t in_features, void* grad_x, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* The SwiGLU experts of qw_moe_experts on microscaled weights and rows:
+ *   h = silu(gate_e(x_s)) * up_e(x_s),  y[s] = down_e(h)
+ * for s in [kept_offsets[e], kept_offsets[e+1]), x_s = x[row_index[s]] (NULL:
+ * x[s]; x has x_rows rows).  x and h are quantised as by qw_mx_quantize (h from
+ * the fp32 sums), products are summed in fp32, y is rounded once to act_dtype.
+ * gate, up: stacks [experts, d_ff, d_model]; down: [experts, d_model, d_ff].
+ * max_rows bounds kept_offsets[experts]; max_rows_per_expert (0: unknown) only
+ * chooses the kernel.  Rows of y that no expert holds are left as they were. */
+size_t qw_mx_experts_workspace_bytes(int64_t x_rows, int64_t max_rows, int64_t experts, int64_t d_model,
+                                     int64_t d_ff);
+int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_stride, const int32_t* row_index,
+                  const int32_t* kept_offsets, int64_t experts, int64_t d_model, int64_t d_ff, int64_t max_rows,
+                  int64_t max_rows_per_expert, const void* gate_codes, const void* gate_scales, const void* up_codes,
+                  const void* up_scales, const void* down_codes, const void* down_scales, void* y, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

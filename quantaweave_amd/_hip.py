@@ -37,3 +37,31 @@ def stream(device: torch.device) -> int:
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """An entry point called with `device` as the current one (a launch goes to
+    the current device, whatever device its stream and tensors are on)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args)
+
+
+_STREAM_KEY = "quantaweave stream"
+
+
+def note_stream(t: torch.Tensor, what: str) -> None:
+    """Called by a differentiable operator before it records a node on `t` (grad
+    mode on, `t` requiring grad).  The node that takes t's gradient is bound to
+    the stream it was first made on and lives as long as any graph through it
+    does.  A backward pass recorded into a HIP graph while it is bound to another
+    stream makes that stream wait inside the capture, which ends the process at
+    the capture's end; so the node is marked with its stream here, and a call
+    under capture that finds another stream's mark is refused."""
+    node = t.view_as(t).grad_fn.next_functions[0][0] if t.grad_fn is None else t.grad_fn
+    here = stream(t.device)
+    if node.metadata.setdefault(_STREAM_KEY, here) != here and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: the input still belongs to a graph made on another stream, so its backward pass "
+                           "cannot be captured; drop that graph's results (or detach the input) before the capture")

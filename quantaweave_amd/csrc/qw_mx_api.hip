@@ -1,0 +1,206 @@
+// C ABI entry points of the microscaled (MX) operators: argument checks,
+// workspace carving and kernel selection.
+#include "qw_mx_product.h"
+
+namespace qw {
+
+int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dtype, int wfmt, int64_t E, int64_t N,
+                            int64_t K, const int32_t* offsets, int64_t rows, int64_t max_rows_per_expert, void* gx,
+                            int accumulate, void* gw, int gw_dtype, void* ws, size_t ws_bytes, hipStream_t stream);
+size_t grouped_backward_workspace_bytes(int64_t E, int64_t N, int64_t K, int64_t rows, int dtype);
+
+namespace {
+
+constexpr int64_t kMaxCols = int64_t{1} << 24;
+
+int check_act(int dtype) {
+  QW_REQUIRE(dtype == QW_F32 || dtype == QW_BF16 || dtype == QW_F16, "dtype must be f32, bf16 or f16");
+  return QW_OK;
+}
+
+int check_sizes(int64_t rows, int64_t out_features, int64_t in_features) {
+  QW_REQUIRE(rows >= 0 && rows <= INT32_MAX / 64, "rows out of range: %lld", (long long)rows);
+  QW_REQUIRE(out_features >= 1 && out_features <= kMaxCols, "out_features out of range: %lld",
+             (long long)out_features);
+  QW_REQUIRE(in_features >= 1 && in_features <= kMaxCols, "in_features out of range: %lld", (long long)in_features);
+  return QW_OK;
+}
+
+int check_matrix(const void* codes, const void* scales, const char* what) {
+  QW_REQUIRE(codes && scales, "%s codes and scales are required", what);
+  QW_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0,
+             "%s codes must start on 16 bytes and its scales on 4", what);
+  return QW_OK;
+}
+
+MxMatrix matrix(const void* codes, const void* scales) {
+  return MxMatrix{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales)};
+}
+
+__global__ void mx_offsets_kernel(int32_t* offsets, int rows) {
+  offsets[0] = 0;
+  offsets[1] = rows;
+}
+
+}  // namespace
+
+}  // namespace qw
+
+using namespace qw;
+
+extern "C" {
+
+int qw_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_row_stride, void* codes,
+                   void* scales, void* stream) {
+  clear_error();
+  int st = check_act(x_dtype);
+  if (st) return st;
+  QW_REQUIRE(rows >= 0, "rows must be >= 0");
+  QW_REQUIRE(cols >= 1 && cols <= kMaxCols, "cols out of range: %lld", (long long)cols);
+  QW_REQUIRE(x_row_stride >= 0, "x_row_stride must be >= 0");
+  if (rows == 0) return QW_OK;
+  QW_REQUIRE(x != nullptr, "x is required");
+  st = check_matrix(codes, scales, "output");
+  if (st) return st;
+  return mx_quantize(x, x_dtype, rows, cols, x_row_stride, codes, scales, as_stream(stream));
+}
+
+int qw_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int out_dtype,
+                     void* stream) {
+  clear_error();
+  int st = check_act(out_dtype);
+  if (st) return st;
+  QW_REQUIRE(rows >= 0, "rows must be >= 0");
+  QW_REQUIRE(cols >= 1 && cols <= kMaxCols, "cols out of range: %lld", (long long)cols);
+  if (rows == 0) return QW_OK;
+  QW_REQUIRE(out != nullptr, "out is required");
+  st = check_matrix(codes, scales, "input");
+  if (st) return st;
+  return mx_dequantize(codes, scales, rows, cols, out, out_dtype, as_stream(stream));
+}
+
+size_t qw_mx_matmul_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features) {
+  (void)rows, (void)out_features, (void)in_features;
+  return 0;
+}
+
+int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t rows, const void* codes,
+                 const void* scales, int64_t out_features, int64_t in_features, void* out, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  clear_error();
+  int st = check_act(act_dtype);
+  if (st) return st;
+  st = check_sizes(rows, out_features, in_features);
+  if (st) return st;
+  QW_REQUIRE(x_row_stride >= 0, "x_row_stride must be >= 0");
+  if (rows == 0) return QW_OK;
+  QW_REQUIRE(x && out, "x and out are required");
+  st = check_matrix(codes, scales, "weight");
+  if (st) return st;
+  (void)workspace, (void)workspace_bytes;
+  MxProduct p;
+  p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride;
+  p.rows = p.row_cap = rows, p.n = out_features, p.k = in_features;
+  p.a = matrix(codes, scales);
+  p.out = out, p.out_dtype = act_dtype;
+  return launch_mx_rows(p, as_stream(stream));
+}
+
+size_t qw_mx_matmul_backward_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features, int dtype) {
+  if (rows < 1 || out_features < 1 || in_features < 1) return 0;
+  Carver c(nullptr);
+  c.take<int32_t>(2);
+  c.take<char>(static_cast<size_t>(out_features) * in_features * (dtype == QW_F32 ? 4 : 2));
+  c.take<char>(grouped_backward_workspace_bytes(1, out_features, in_features, rows, dtype));
+  return c.used + 256;
+}
+
+int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const void* codes, const void* scales,
+                          int64_t out_features, int64_t in_features, void* grad_x, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  clear_error();
+  int st = check_act(dtype);
+  if (st) return st;
+  st = check_sizes(rows, out_features, in_features);
+  if (st) return st;
+  if (rows == 0) return QW_OK;
+  QW_REQUIRE(grad_out && grad_x, "grad_out and grad_x are required");
+  st = check_matrix(codes, scales, "weight");
+  if (st) return st;
+  const size_t need = qw_mx_matmul_backward_workspace_bytes(rows, out_features, in_features, dtype);
+  if (workspace == nullptr || workspace_bytes < need)
+    return set_error(QW_ERR_WORKSPACE, "mx_matmul_backward needs a workspace of %zu bytes, got %zu", need,
+                     workspace_bytes);
+  Carver c(workspace);
+  int32_t* offsets = c.take<int32_t>(2);
+  void* w = c.take<char>(static_cast<size_t>(out_features) * in_features * (dtype == QW_F32 ? 4 : 2));
+  const size_t inner = grouped_backward_workspace_bytes(1, out_features, in_features, rows, dtype);
+  void* ws = c.take<char>(inner);
+  mx_offsets_kernel<<<1, 1, 0, as_stream(stream)>>>(offsets, static_cast<int>(rows));
+  QW_LAUNCH_CHECK("mx_offsets_kernel");
+  st = mx_dequantize(codes, scales, out_features, in_features, w, dtype, as_stream(stream));
+  if (st) return st;
+  return grouped_matmul_backward(grad_out, nullptr, w, dtype, dtype, 1, out_features, in_features, offsets, rows, rows,
+                                 grad_x, 0, nullptr, dtype, ws, inner, as_stream(stream));
+}
+
+size_t qw_mx_experts_workspace_bytes(int64_t x_rows, int64_t max_rows, int64_t experts, int64_t d_model,
+                                     int64_t d_ff) {
+  if (x_rows < 0 || max_rows < 0 || experts < 1 || d_model < 1 || d_ff < 1) return 0;
+  Carver c(nullptr);
+  c.take<char>(static_cast<size_t>(x_rows) * mx_code_bytes(d_model));
+  c.take<char>(static_cast<size_t>(x_rows) * mx_scale_bytes(d_model));
+  c.take<char>(static_cast<size_t>(max_rows) * mx_code_bytes(d_ff));
+  c.take<char>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_ff));
+  return c.used + 256;
+}
+
+int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_stride, const int32_t* row_index,
+                  const int32_t* kept_offsets, int64_t experts, int64_t d_model, int64_t d_ff, int64_t max_rows,
+                  int64_t max_rows_per_expert, const void* gate_codes, const void* gate_scales, const void* up_codes,
+                  const void* up_scales, const void* down_codes, const void* down_scales, void* y, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  clear_error();
+  int st = check_act(act_dtype);
+  if (st) return st;
+  st = check_sizes(max_rows, d_ff, d_model);
+  if (st) return st;
+  QW_REQUIRE(experts >= 1 && experts <= 65535, "experts out of range: %lld", (long long)experts);
+  QW_REQUIRE(x_rows >= 0 && x_rows <= INT32_MAX / 64, "x_rows out of range: %lld", (long long)x_rows);
+  QW_REQUIRE(row_index != nullptr || x_rows >= max_rows, "x has %lld rows for %lld", (long long)x_rows,
+             (long long)max_rows);
+  QW_REQUIRE(x_row_stride >= 0 && max_rows_per_expert >= 0, "strides and bounds must be >= 0");
+  if (max_rows == 0 || x_rows == 0) return QW_OK;
+  QW_REQUIRE(x && y && kept_offsets, "x, y and kept_offsets are required");
+  st = check_matrix(gate_codes, gate_scales, "gate");
+  if (!st) st = check_matrix(up_codes, up_scales, "up");
+  if (!st) st = check_matrix(down_codes, down_scales, "down");
+  if (st) return st;
+  const size_t need = qw_mx_experts_workspace_bytes(x_rows, max_rows, experts, d_model, d_ff);
+  if (workspace == nullptr || workspace_bytes < need)
+    return set_error(QW_ERR_WORKSPACE, "mx_experts needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
+  Carver c(workspace);
+  uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(x_rows) * mx_code_bytes(d_model));
+  uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(x_rows) * mx_scale_bytes(d_model));
+  uint8_t* hq = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_code_bytes(d_ff));
+  uint8_t* hs = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_ff));
+  (void)xq, (void)xs;
+  MxProduct p;
+  p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride, p.row_index = row_index;
+  p.offsets = kept_offsets, p.groups = experts, p.rows = max_rows;
+  p.row_cap = max_rows_per_expert > 0 && max_rows_per_expert < max_rows ? max_rows_per_expert : max_rows;
+  p.n = d_ff, p.k = d_model;
+  p.a = matrix(gate_codes, gate_scales), p.b = matrix(up_codes, up_scales);
+  p.h_codes = hq, p.h_scales = hs;
+  st = launch_mx_rows(p, as_stream(stream));
+  if (st) return st;
+  MxProduct d;
+  d.x_codes = hq, d.x_scales = hs;
+  d.offsets = kept_offsets, d.groups = experts, d.rows = max_rows, d.row_cap = p.row_cap;
+  d.n = d_model, d.k = d_ff;
+  d.a = matrix(down_codes, down_scales);
+  d.out = y, d.out_dtype = act_dtype;
+  return launch_mx_rows(d, as_stream(stream));
+}
+
+}  // extern "C"

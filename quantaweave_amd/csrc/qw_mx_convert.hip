@@ -1,0 +1,112 @@
+// Rows of numbers <-> microscaled rows (qw_mx.h).
+#include "qw_mx.h"
+
+namespace qw {
+
+namespace {
+
+constexpr int kConvertThreads = 256;
+
+// Four lanes make a block: each loads eight consecutive numbers (16 bytes of a
+// 16-bit type), the largest magnitude goes round the four with two DPP moves,
+// each stores four bytes of codes and the first the scale byte.  Padding columns
+// are written as zeros.  Bound by HBM.
+template <int DT>
+__global__ __launch_bounds__(kConvertThreads) void mx_quantize_kernel(const void* __restrict__ x, int64_t stride,
+                                                                      int cols, uint32_t pieces, int64_t total,
+                                                                      bool aligned, uint32_t* __restrict__ codes,
+                                                                      uint8_t* __restrict__ scales) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvertThreads + threadIdx.x;
+  if (i >= total) return;  // whole blocks: total is a multiple of 16 and the four lanes of a block go together
+  const int64_t row = total <= INT32_MAX ? static_cast<uint32_t>(i) / pieces : i / pieces;
+  const int col = static_cast<int>(i - row * pieces) * 8;
+  const MxPiece<DT> v = mx_load_piece<DT>(x, row * stride + col, cols - col, aligned);
+  uint32_t top = mx_piece_top<DT>(v);
+  top = mx_top_max<DT>(top, dpp_u32<kDppXor1>(top));
+  top = mx_top_max<DT>(top, dpp_u32<kDppXor2>(top));
+  const uint32_t s = mx_scale_of(mx_top_bits<DT>(top));
+  codes[i] = mx_piece_codes<DT>(v, s);
+  if (threadIdx.x % 4 == 0) scales[i / 4] = static_cast<uint8_t>(s);
+}
+
+// A lane turns four bytes of codes into eight numbers: code times scale is exact
+// in fp32 (subnormals included) and is rounded once to the output type.
+template <int DT>
+__global__ __launch_bounds__(kConvertThreads) void mx_dequantize_kernel(const uint32_t* __restrict__ codes,
+                                                                        const uint8_t* __restrict__ scales, int cols,
+                                                                        uint32_t pieces, int64_t total, bool aligned,
+                                                                        void* __restrict__ out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvertThreads + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = total <= INT32_MAX ? static_cast<uint32_t>(i) / pieces : i / pieces;
+  const int col = static_cast<int>(i - row * pieces) * 8;
+  if (col >= cols) return;
+  const float s = mx_scale_value(scales[i / 4]);
+  const uint32_t c = codes[i];
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  const f32x2_t p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3)};
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = p[k / 2][k % 2] * s;
+  const int64_t o = row * cols + col;
+  if (aligned && col + 8 <= cols) {
+    store_vec<DT, 8>(out, o, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (col + k < cols) store_act<DT>(out, o + k, v[k]);
+  }
+}
+
+}  // namespace
+
+int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
+                hipStream_t stream) {
+  const int64_t pieces = mx_padded(cols) / 8, total = rows * pieces;
+  if (total == 0) return QW_OK;
+  const int64_t blocks = ceil_div(total, kConvertThreads);
+  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many rows to quantise in one call");
+  const int size = dtype == QW_F32 ? 4 : 2;
+  const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * size % 16 == 0;
+  const unsigned g = static_cast<unsigned>(blocks);
+  const int c = static_cast<int>(cols);
+  const uint32_t p = static_cast<uint32_t>(pieces);
+  uint32_t* q = static_cast<uint32_t*>(codes);
+  uint8_t* s = static_cast<uint8_t*>(scales);
+  if (dtype == QW_F32)
+    mx_quantize_kernel<QW_F32><<<g, kConvertThreads, 0, stream>>>(x, stride, c, p, total, aligned, q, s);
+  else if (dtype == QW_F16)
+    mx_quantize_kernel<QW_F16><<<g, kConvertThreads, 0, stream>>>(x, stride, c, p, total, aligned, q, s);
+  else
+    mx_quantize_kernel<QW_BF16><<<g, kConvertThreads, 0, stream>>>(x, stride, c, p, total, aligned, q, s);
+  QW_LAUNCH_CHECK("mx_quantize_kernel");
+  return QW_OK;
+}
+
+int mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
+                  hipStream_t stream) {
+  const int64_t pieces = mx_padded(cols) / 8, total = rows * pieces;
+  if (total == 0) return QW_OK;
+  const int64_t blocks = ceil_div(total, kConvertThreads);
+  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many rows to dequantise in one call");
+  const int size = dtype == QW_F32 ? 4 : 2;
+  const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && cols * size % 16 == 0;
+  const unsigned g = static_cast<unsigned>(blocks);
+  const int c = static_cast<int>(cols);
+  const uint32_t p = static_cast<uint32_t>(pieces);
+  const uint32_t* q = static_cast<const uint32_t*>(codes);
+  const uint8_t* s = static_cast<const uint8_t*>(scales);
+  if (dtype == QW_F32)
+    mx_dequantize_kernel<QW_F32><<<g, kConvertThreads, 0, stream>>>(q, s, c, p, total, aligned, out);
+  else if (dtype == QW_F16)
+    mx_dequantize_kernel<QW_F16><<<g, kConvertThreads, 0, stream>>>(q, s, c, p, total, aligned, out);
+  else
+    mx_dequantize_kernel<QW_BF16><<<g, kConvertThreads, 0, stream>>>(q, s, c, p, total, aligned, out);
+  QW_LAUNCH_CHECK("mx_dequantize_kernel");
+  return QW_OK;
+}
+
+}  // namespace qw

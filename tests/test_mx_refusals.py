@@ -1,0 +1,108 @@
+"""What the microscaled operators and the scored routing refuse, and the oracle they are tested against (CPU only)."""
+
+import pytest
+import torch
+
+import quantaweave_amd as qa
+from quantaweave_amd import _lib
+from quantaweave_amd.routing import check_rule
+from tests import mx_oracle as ref
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(4, 64)
+    codes, scales = ref.stored(torch.Generator().manual_seed(0), 8, 64)
+    for call in (lambda: qa.mx_quantize(x), lambda: qa.mx_dequantize(codes, scales, 64),
+                 lambda: qa.mx_matmul(x, codes, scales), lambda: qa.route_experts(x, 2),
+                 lambda: qa.mx_grouped_swiglu(x, (codes, scales), (codes, scales), (codes, scales), torch.zeros(2).int())):
+        with pytest.raises(RuntimeError, match="ROCm"):
+            call()
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(score="tanh"), "score"), (dict(group_score="sum"), "group_score"), (dict(experts=0), "experts"),
+    (dict(experts=1025), "experts"), (dict(groups=0), "groups"), (dict(groups=5), "groups"),
+    (dict(top_groups=9), "top_groups"), (dict(top_k=0), "top_k"), (dict(top_k=33), "top_k"),
+    (dict(experts=256, groups=1, top_groups=1, top_k=65), "top_k"), (dict(scale=float("nan")), "scale")])
+def test_rules_that_no_kernel_takes(change, match):
+    rule = dict(experts=64, top_k=8, score="sigmoid", groups=8, top_groups=4, group_score="top2", scale=1.0)
+    check_rule(**rule)
+    with pytest.raises(ValueError, match=match):
+        check_rule(**{**rule, **change})
+
+
+def test_entry_points_check_their_arguments_before_any_launch():
+    lib = _lib.load()
+    one = 64  # an address that is never read: the calls below are refused before a launch
+
+    def refused(status, word):
+        assert status == _lib.QW_ERR_INVALID and word in lib.qw_last_error(), lib.qw_last_error()
+
+    route = lib.qw_moe_route_scored_from_logits
+    refused(route(one, 4, 64, 65, 0, None, 1, 1, 2, 1, 1.0, one, None, one, one, None), b"top_k")
+    refused(route(one, 4, 64, 2, 2, None, 1, 1, 2, 1, 1.0, one, None, one, one, None), b"score")
+    refused(route(one, 4, 64, 2, 0, None, 7, 1, 2, 1, 1.0, one, None, one, one, None), b"groups")
+    refused(route(one, 4, 64, 2, 0, None, 8, 9, 2, 1, 1.0, one, None, one, one, None), b"top_groups")
+    refused(route(one, 4, 64, 9, 0, None, 8, 1, 2, 1, 1.0, one, None, one, one, None), b"top_k")
+    refused(route(one, 4, 64, 2, 0, None, 8, 1, 3, 1, 1.0, one, None, one, one, None), b"group_top")
+    refused(route(None, 4, 64, 2, 0, None, 8, 1, 2, 1, 1.0, one, None, one, one, None), b"logits")
+    refused(lib.qw_moe_route_scored_backward(one, one, one, None, None, one, None, 4, 8, 2, 0, 1, 1.0, 1.0, one, None),
+            b"counts")
+    refused(lib.qw_moe_route_scored_backward(one, one, one, None, None, None, None, 4, 8, 2, 0, 1, 1.0, 0.0, one, None),
+            b"temperature")
+    refused(lib.qw_mx_quantize(one, 7, 4, 64, 64, one, one, None), b"dtype")
+    refused(lib.qw_mx_quantize(one, 0, 4, 0, 64, one, one, None), b"cols")
+    refused(lib.qw_mx_quantize(one, 0, 4, 64, -1, one, one, None), b"stride")
+    refused(lib.qw_mx_quantize(one, 0, 4, 64, 64, 72, one, None), b"16 bytes")
+    refused(lib.qw_mx_dequantize(one, 66, 4, 64, one, 0, None), b"on 4")
+    refused(lib.qw_mx_matmul(one, 1, 64, 4, None, one, 8, 64, one, None, 0, None), b"weight")
+    refused(lib.qw_mx_matmul(one, 1, 64, -1, one, one, 8, 64, one, None, 0, None), b"rows")
+    refused(lib.qw_mx_experts(one, 1, 3, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, one, one, 1 << 30,
+                              None), b"rows")
+    refused(lib.qw_mx_experts(one, 1, 4, 64, None, one, 0, 64, 64, 4, 0, one, one, one, one, one, one, one, one, 1 << 30,
+                              None), b"experts")
+    need = lib.qw_mx_experts_workspace_bytes(4, 4, 2, 64, 64)
+    assert lib.qw_mx_experts(one, 1, 4, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, one, one,
+                             need - 1, None) == _lib.QW_ERR_WORKSPACE
+    need = lib.qw_mx_matmul_backward_workspace_bytes(4, 8, 64, 1)
+    assert lib.qw_mx_matmul_backward(one, 1, 4, one, one, 8, 64, one, one, need - 1, None) == _lib.QW_ERR_WORKSPACE
+    # nothing to do is no error
+    assert lib.qw_mx_quantize(None, 0, 0, 64, 64, None, None, None) == _lib.QW_OK
+    assert route(None, 0, 64, 2, 0, None, 8, 1, 2, 1, 1.0, None, None, None, None, None) == _lib.QW_OK
+
+
+def test_oracle_rounds_to_the_nearest_value_with_ties_to_even():
+    x = torch.tensor([[0.25, 0.26, 0.75, 0.74, 1.25, 1.75, 2.5, 3.5, 5.0, 5.01, 7.9, -0.25, -2.5, 4.0] + [0.0] * 18])
+    want = [0, 0.5, 1, 0.5, 1, 2, 2, 4, 4, 6, 6, 0, -2, 4] + [0.0] * 18
+    assert ref.on_grid(x)[0].tolist() == want
+    assert ref.quantize(x)[1].tolist() == [[127, 0, 0, 0]]
+
+
+def test_oracle_values_and_quantise_are_inverse():
+    codes, scales = ref.stored(torch.Generator().manual_seed(3), 5, 256)
+    codes[:, ::16] = 0x77  # every block reaches 6, so its scale is the stored one
+    v = ref.values(codes, scales, 256)
+    assert torch.equal(ref.on_grid(v), v)
+
+
+def test_backward_under_capture_is_refused_while_a_graph_of_another_stream_lives(monkeypatch):
+    """The streams and the capture are stood in for: the refusal is decided on the host, before any launch."""
+    from quantaweave_amd import _hip
+
+    now = {"stream": 1, "capturing": False}
+    monkeypatch.setattr(_hip, "stream", lambda device: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    leaf = torch.randn(3, requires_grad=True)
+    for t in (leaf, leaf * 2):
+        now.update(stream=1, capturing=False)
+        _hip.note_stream(t, "op")
+        kept = t * 2  # the eager graph
+        now.update(stream=7, capturing=True)
+        with pytest.raises(RuntimeError, match="another stream"):
+            _hip.note_stream(t, "op")
+        now.update(stream=1)
+        _hip.note_stream(t, "op")  # captured on the stream the graph was made on
+        del kept
+    del t
+    now.update(stream=7)
+    _hip.note_stream(leaf, "op")  # the graph is gone, and its node with it
