@@ -80,8 +80,11 @@ int qw_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_
 }
 
 size_t qw_mx_matmul_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features) {
-  (void)rows, (void)out_features, (void)in_features;
-  return 0;
+  if (rows < 1 || out_features < 1 || in_features < 1 || mx_few_rows(rows, 1)) return 0;
+  Carver c(nullptr);
+  c.take<char>(static_cast<size_t>(rows) * mx_code_bytes(in_features));
+  c.take<char>(static_cast<size_t>(rows) * mx_scale_bytes(in_features));
+  return c.used + 256;
 }
 
 int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t rows, const void* codes,
@@ -97,13 +100,24 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
   QW_REQUIRE(x && out, "x and out are required");
   st = check_matrix(codes, scales, "weight");
   if (st) return st;
-  (void)workspace, (void)workspace_bytes;
+  const size_t need = qw_mx_matmul_workspace_bytes(rows, out_features, in_features);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return set_error(QW_ERR_WORKSPACE, "mx_matmul needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
   MxProduct p;
-  p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride;
   p.rows = p.row_cap = rows, p.n = out_features, p.k = in_features;
   p.a = matrix(codes, scales);
   p.out = out, p.out_dtype = act_dtype;
-  return launch_mx_rows(p, as_stream(stream));
+  if (need == 0) {
+    p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride;
+    return launch_mx_rows(p, as_stream(stream));
+  }
+  Carver c(workspace);
+  uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(rows) * mx_code_bytes(in_features));
+  uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(rows) * mx_scale_bytes(in_features));
+  st = mx_quantize(x, act_dtype, rows, in_features, x_row_stride, xq, xs, as_stream(stream));
+  if (st) return st;
+  p.x_codes = xq, p.x_scales = xs;
+  return launch_mx_gemm(p, as_stream(stream));
 }
 
 size_t qw_mx_matmul_backward_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features, int dtype) {
@@ -184,15 +198,22 @@ int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_st
   uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(x_rows) * mx_scale_bytes(d_model));
   uint8_t* hq = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_code_bytes(d_ff));
   uint8_t* hs = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_ff));
-  (void)xq, (void)xs;
+  const bool few = mx_few_rows(max_rows, experts);
   MxProduct p;
-  p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride, p.row_index = row_index;
+  p.row_index = row_index, p.x_rows = x_rows;
+  if (few) {
+    p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride;
+  } else {
+    st = mx_quantize(x, act_dtype, x_rows, d_model, x_row_stride, xq, xs, as_stream(stream));
+    if (st) return st;
+    p.x_codes = xq, p.x_scales = xs;
+  }
   p.offsets = kept_offsets, p.groups = experts, p.rows = max_rows;
   p.row_cap = max_rows_per_expert > 0 && max_rows_per_expert < max_rows ? max_rows_per_expert : max_rows;
   p.n = d_ff, p.k = d_model;
   p.a = matrix(gate_codes, gate_scales), p.b = matrix(up_codes, up_scales);
   p.h_codes = hq, p.h_scales = hs;
-  st = launch_mx_rows(p, as_stream(stream));
+  st = few ? launch_mx_rows(p, as_stream(stream)) : launch_mx_gemm(p, as_stream(stream));
   if (st) return st;
   MxProduct d;
   d.x_codes = hq, d.x_scales = hs;
@@ -200,7 +221,7 @@ int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_st
   d.n = d_model, d.k = d_ff;
   d.a = matrix(down_codes, down_scales);
   d.out = y, d.out_dtype = act_dtype;
-  return launch_mx_rows(d, as_stream(stream));
+  return few ? launch_mx_rows(d, as_stream(stream)) : launch_mx_gemm(d, as_stream(stream));
 }
 
 }  // extern "C"

@@ -26,7 +26,7 @@ struct MxProduct {
   const uint8_t* x_scales = nullptr;
   const int32_t* row_index = nullptr;
   const int32_t* offsets = nullptr;
-  int64_t groups = 1, rows = 0, row_cap = 0, n = 0, k = 0;
+  int64_t groups = 1, rows = 0, x_rows = 0, row_cap = 0, n = 0, k = 0;  // x_rows: rows behind row_index
   MxMatrix a{nullptr, nullptr}, b{nullptr, nullptr};
   void* out = nullptr;
   int out_dtype = QW_F32;
@@ -36,6 +36,11 @@ struct MxProduct {
 
 // Few rows per group: weights streamed, K split over the waves of a workgroup.
 int launch_mx_rows(const MxProduct& p, hipStream_t stream);
+// Many rows (stored ones): tiles of the matrix instruction through LDS.
+int launch_mx_gemm(const MxProduct& p, hipStream_t stream);
+
+// Whether a product of `rows` rows in `groups` groups is one of few rows.
+inline bool mx_few_rows(int64_t rows, int64_t groups) { return rows <= groups * 16; }
 
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
                 hipStream_t stream);
