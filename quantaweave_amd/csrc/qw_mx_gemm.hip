@@ -173,10 +173,11 @@ __global__ __launch_bounds__(MX_THREADS) void mx_gemm_kernel(
   for (int i = 0; i < SUBT; ++i)
 #pragma unroll
     for (int t = 0; t < MX_NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int brow[MX_NT];
-#pragma unroll
-  for (int t = 0; t < MX_NT; ++t)
-    brow[t] = GATEUP ? (t < MX_NT / 2 ? 0 : MX_NB / 2) + wn * 32 + (t % (MX_NT / 2)) * 16 : wn * 64 + t * 16;
+  // this lane's fragment in a stage: its row of sub-tile wm, of weight tile 0, and their scales
+  const int frag = l16 * MX_SLICE + mx_swz(l16, lq) * 16;
+  const int b_row = wn * (GATEUP ? 32 : 64);
+  const int a_lane = wm * 16 * MX_SLICE + frag, b_lane = b_row * MX_SLICE + frag;
+  const int as_lane = (wm * 16 + l16) * MX_SROW + lq, bs_lane = (b_row + l16) * MX_SROW + lq;
   const int active_sub = (count + 15) / 16;
 
   for (int s = 0; s < AHEAD && s < KT; ++s) issue(s);
@@ -190,17 +191,27 @@ __global__ __launch_bounds__(MX_THREADS) void mx_gemm_kernel(
   };
   auto slice = [&](auto npa, auto steps, const char* st, auto&& request) {
     constexpr int NPA = decltype(npa)::value, STEPS = decltype(steps)::value;
-    const char* const st_b = st + A_STAGE;
-    const char* const st_as = st_b + B_STAGE;
-    const char* const st_bs = st_as + AS_STAGE;
-    auto read = [&](const char* codes, const char* scales, int row, int ks) {
+    // one address per step and operand, the rest are constant offsets: a row's swizzle
+    // is that of its lane, and the second step's pieces lie 64 bytes across
+    const char* const a0 = st + a_lane;
+    const char* const a1 = st + (a_lane ^ 64);
+    const char* const b0 = st + A_STAGE + b_lane;
+    const char* const b1 = st + A_STAGE + (b_lane ^ 64);
+    const char* const as = st + A_STAGE + B_STAGE + as_lane;
+    const char* const bs = st + A_STAGE + B_STAGE + AS_STAGE + bs_lane;
+    auto read_a = [&](int i, int ks) {
       Frag f;
-      f.v = *reinterpret_cast<const u32x4*>(codes + row * MX_SLICE + mx_swz(row, lq + 4 * ks) * 16);
-      f.s = *reinterpret_cast<const uint8_t*>(scales + row * MX_SROW + ks * 4 + lq);
+      f.v = *reinterpret_cast<const u32x4*>((ks ? a1 : a0) + i * 32 * MX_SLICE);
+      f.s = *reinterpret_cast<const uint8_t*>(as + i * 32 * MX_SROW + ks * 4);
       return f;
     };
-    auto read_a = [&](int i, int ks) { return read(st, st_as, (wm + 2 * i) * 16 + l16, ks); };
-    auto read_b = [&](int t, int ks) { return read(st_b, st_bs, brow[t] + l16, ks); };
+    auto read_b = [&](int t, int ks) {
+      const int row = GATEUP ? t / 2 * (MX_NB / 2) + t % 2 * 16 : t * 16;
+      Frag f;
+      f.v = *reinterpret_cast<const u32x4*>((ks ? b1 : b0) + row * MX_SLICE);
+      f.s = *reinterpret_cast<const uint8_t*>(bs + row * MX_SROW + ks * 4);
+      return f;
+    };
     Frag w[2][MX_NT], xb[2][2];
 #pragma unroll
     for (int t = 0; t < MX_NT; ++t) w[0][t] = read_b(t, 0);
@@ -241,19 +252,23 @@ __global__ __launch_bounds__(MX_THREADS) void mx_gemm_kernel(
   auto k_loop = [&](auto npa) {
     using Two = std::integral_constant<int, 2>;
     using One = std::integral_constant<int, 1>;
-    const int full = half ? KT - 1 : KT;
-    for (int kt = 0; kt < full; ++kt) {
+    // slice kt has landed when only the slices requested after it may be in flight
+    int kt = 0;
+    for (; kt < KT - AHEAD; ++kt) {
+      wait_vmcnt<(AHEAD - 1) * LOADS>();
+      ring_barrier();
+      slice(npa, Two{}, smem + (kt % ST) * STAGE, [&] { issue(kt + AHEAD); });
+    }
+    for (const int full = half ? KT - 1 : KT; kt < full; ++kt) {
       if (AHEAD == 2 && kt + 1 < KT) wait_vmcnt<LOADS>();
       else wait_vmcnt<0>();
       ring_barrier();
-      slice(npa, Two{}, smem + (kt % ST) * STAGE, [&] {
-        if (kt + AHEAD < KT) issue(kt + AHEAD);
-      });
+      slice(npa, Two{}, smem + (kt % ST) * STAGE, [] {});
     }
     if (half) {
       wait_vmcnt<0>();
       ring_barrier();
-      slice(npa, One{}, smem + (full % ST) * STAGE, [] {});
+      slice(npa, One{}, smem + (kt % ST) * STAGE, [] {});
     }
   };
   const int wave_sub = active_sub > wm ? (active_sub - wm + 1) / 2 : 0;
