@@ -549,14 +549,14 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
  * the fp32 sums), products are summed in fp32, y is rounded once to act_dtype.
  * gate, up: stacks [experts, d_ff, d_model]; down: [experts, d_model, d_ff].
  * max_rows bounds kept_offsets[experts]; max_rows_per_expert (0: unknown) only
- * chooses the kernel.  Rows of y that no expert holds are left as they were. */
-size_t qw_mx_experts_workspace_bytes(int64_t x_rows, int64_t max_rows, int64_t experts, int64_t d_model,
-                                     int64_t d_ff);
+ * chooses the kernel.  Rows of y past kept_offsets[experts] are left as they were,
+ * or become zeros where zero_rest != 0. */
+size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t d_model, int64_t d_ff);
 int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_stride, const int32_t* row_index,
                   const int32_t* kept_offsets, int64_t experts, int64_t d_model, int64_t d_ff, int64_t max_rows,
                   int64_t max_rows_per_expert, const void* gate_codes, const void* gate_scales, const void* up_codes,
-                  const void* up_scales, const void* down_codes, const void* down_scales, void* y, void* workspace,
-                  size_t workspace_bytes, void* stream);
+                  const void* up_scales, const void* down_codes, const void* down_scales, int zero_rest, void* y,
+                  void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

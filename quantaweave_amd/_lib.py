@@ -82,8 +82,8 @@ SIGNATURES = {
     "qw_mx_matmul": (I32, [P, I32, I64, I64, P, P, I64, I64, P, P, SZ, P]),
     "qw_mx_matmul_backward_workspace_bytes": (SZ, [I64, I64, I64, I32]),
     "qw_mx_matmul_backward": (I32, [P, I32, I64, P, P, I64, I64, P, P, SZ, P]),
-    "qw_mx_experts_workspace_bytes": (SZ, [I64, I64, I64, I64, I64]),
-    "qw_mx_experts": (I32, [P, I32, I64, I64, P, P, I64, I64, I64, I64, I64, P, P, P, P, P, P, P, P, SZ, P]),
+    "qw_mx_experts_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+    "qw_mx_experts": (I32, [P, I32, I64, I64, P, P, I64, I64, I64, I64, I64, P, P, P, P, P, P, I32, P, P, SZ, P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -26,18 +26,37 @@ inline int64_t mx_padded(int64_t cols) { return ceil_div(cols, kMxStep) * kMxSte
 inline int64_t mx_code_bytes(int64_t cols) { return mx_padded(cols) / 2; }
 inline int64_t mx_scale_bytes(int64_t cols) { return mx_padded(cols) / kMxBlock; }
 
+// Lanes of a wave have written LDS that others of it read next (or the reverse):
+// the wave's LDS accesses are in order, the compiler has to keep them so.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+}
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// acc += the product of a step: 16 rows of a (accumulator rows), 16 rows of b
-// (accumulator columns).  Scales in byte 0 of sa and sb.  The products are exact
-// and are added in fp32.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ i32x8 mx_operand(u32x4 v) {
+  return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
+}
+
+// acc += the product of 128 columns: 16 rows of a (accumulator rows), 16 rows of b
+// (accumulator columns); lane l holds block l / 16 of row l % 16.  Scales in byte
+// 0 of sa and sb.  The products are exact and are added in fp32.
 __device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 acc, uint32_t sa, uint32_t sb) {
-  const i32x8 av = {static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]),
-                    0, 0, 0, 0};
-  const i32x8 bv = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]),
-                    0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, static_cast<int>(sa), 0,
-                                                          static_cast<int>(sb));
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(a), mx_operand(b), acc, 4, 4, 0,
+                                                          static_cast<int>(sa), 0, static_cast<int>(sb));
+}
+
+// The same for 64 columns of 32 by 32 rows: lane l holds block l / 32 of row
+// l % 32, scales in byte BYTE; accumulator element e of a lane is row
+// 8 (e / 4) + 4 (l / 32) + e % 4 of a, row l % 32 of b.
+template <int BYTE>
+__device__ __forceinline__ f32x16 mx_mfma32(u32x4 a, u32x4 b, f32x16 acc, uint32_t sa, uint32_t sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a), mx_operand(b), acc, 4, 4, BYTE,
+                                                         static_cast<int>(sa), BYTE, static_cast<int>(sb));
 }
 
 // Scale byte of a block from the fp32 bits of its largest magnitude.

@@ -104,7 +104,7 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return set_error(QW_ERR_WORKSPACE, "mx_matmul needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
   MxProduct p;
-  p.rows = p.row_cap = rows, p.n = out_features, p.k = in_features;
+  p.rows = rows, p.n = out_features, p.k = in_features;
   p.a = matrix(codes, scales);
   p.out = out, p.out_dtype = act_dtype;
   if (need == 0) {
@@ -114,9 +114,10 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
   Carver c(workspace);
   uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(rows) * mx_code_bytes(in_features));
   uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(rows) * mx_scale_bytes(in_features));
-  st = mx_quantize(x, act_dtype, rows, in_features, x_row_stride, xq, xs, as_stream(stream));
+  st = mx_prepare(x, act_dtype, rows, in_features, x_row_stride, xq, xs, MxPrepare(), as_stream(stream));
   if (st) return st;
   p.x_codes = xq, p.x_scales = xs;
+  p.chunk_rows = mx_dense_chunk(rows, out_features);
   return launch_mx_gemm(p, as_stream(stream));
 }
 
@@ -158,22 +159,24 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
                                  grad_x, 0, nullptr, dtype, ws, inner, as_stream(stream));
 }
 
-size_t qw_mx_experts_workspace_bytes(int64_t x_rows, int64_t max_rows, int64_t experts, int64_t d_model,
-                                     int64_t d_ff) {
-  if (x_rows < 0 || max_rows < 0 || experts < 1 || d_model < 1 || d_ff < 1) return 0;
+size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t d_model, int64_t d_ff) {
+  if (max_rows < 0 || experts < 1 || d_model < 1 || d_ff < 1) return 0;
   Carver c(nullptr);
-  c.take<char>(static_cast<size_t>(x_rows) * mx_code_bytes(d_model));
-  c.take<char>(static_cast<size_t>(x_rows) * mx_scale_bytes(d_model));
   c.take<char>(static_cast<size_t>(max_rows) * mx_code_bytes(d_ff));
   c.take<char>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_ff));
+  if (!mx_few_rows(max_rows, experts)) {
+    c.take<char>(static_cast<size_t>(max_rows) * mx_code_bytes(d_model));
+    c.take<char>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_model));
+    c.take<int4>(static_cast<size_t>(mx_max_chunks(max_rows, experts, 64)) + 1);  // the smallest chunks
+  }
   return c.used + 256;
 }
 
 int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_stride, const int32_t* row_index,
                   const int32_t* kept_offsets, int64_t experts, int64_t d_model, int64_t d_ff, int64_t max_rows,
                   int64_t max_rows_per_expert, const void* gate_codes, const void* gate_scales, const void* up_codes,
-                  const void* up_scales, const void* down_codes, const void* down_scales, void* y, void* workspace,
-                  size_t workspace_bytes, void* stream) {
+                  const void* up_scales, const void* down_codes, const void* down_scales, int zero_rest, void* y,
+                  void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   int st = check_act(act_dtype);
   if (st) return st;
@@ -190,38 +193,41 @@ int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_st
   if (!st) st = check_matrix(up_codes, up_scales, "up");
   if (!st) st = check_matrix(down_codes, down_scales, "down");
   if (st) return st;
-  const size_t need = qw_mx_experts_workspace_bytes(x_rows, max_rows, experts, d_model, d_ff);
+  const size_t need = qw_mx_experts_workspace_bytes(max_rows, experts, d_model, d_ff);
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(QW_ERR_WORKSPACE, "mx_experts needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
   Carver c(workspace);
-  uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(x_rows) * mx_code_bytes(d_model));
-  uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(x_rows) * mx_scale_bytes(d_model));
-  uint8_t* hq = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_code_bytes(d_ff));
-  uint8_t* hs = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_ff));
-  const bool few = mx_few_rows(max_rows, experts);
-  MxProduct p;
-  p.row_index = row_index, p.x_rows = x_rows;
-  if (few) {
-    p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride;
-  } else {
-    st = mx_quantize(x, act_dtype, x_rows, d_model, x_row_stride, xq, xs, as_stream(stream));
-    if (st) return st;
-    p.x_codes = xq, p.x_scales = xs;
-  }
+  MxProduct p, d;
+  p.h_codes = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_code_bytes(d_ff));
+  p.h_scales = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_ff));
   p.offsets = kept_offsets, p.groups = experts, p.rows = max_rows;
-  p.row_cap = max_rows_per_expert > 0 && max_rows_per_expert < max_rows ? max_rows_per_expert : max_rows;
   p.n = d_ff, p.k = d_model;
   p.a = matrix(gate_codes, gate_scales), p.b = matrix(up_codes, up_scales);
-  p.h_codes = hq, p.h_scales = hs;
-  st = few ? launch_mx_rows(p, as_stream(stream)) : launch_mx_gemm(p, as_stream(stream));
-  if (st) return st;
-  MxProduct d;
-  d.x_codes = hq, d.x_scales = hs;
-  d.offsets = kept_offsets, d.groups = experts, d.rows = max_rows, d.row_cap = p.row_cap;
+  d.x_codes = p.h_codes, d.x_scales = p.h_scales;
+  d.offsets = kept_offsets, d.groups = experts, d.rows = max_rows;
   d.n = d_model, d.k = d_ff;
   d.a = matrix(down_codes, down_scales);
   d.out = y, d.out_dtype = act_dtype;
-  return few ? launch_mx_rows(d, as_stream(stream)) : launch_mx_gemm(d, as_stream(stream));
+  if (mx_few_rows(max_rows, experts)) {
+    p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride, p.row_index = row_index;
+    st = launch_mx_rows(p, as_stream(stream));
+    d.zero_rest = zero_rest != 0;
+    return st ? st : launch_mx_rows(d, as_stream(stream));
+  }
+  uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_code_bytes(d_model));
+  uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_model));
+  const int64_t cap = max_rows_per_expert > 0 && max_rows_per_expert < max_rows ? max_rows_per_expert : max_rows;
+  MxPrepare prep;
+  prep.row_index = row_index, prep.offsets = kept_offsets, prep.groups = experts;
+  prep.chunk_rows = p.chunk_rows = d.chunk_rows = mx_group_chunk(max_rows, experts, cap);
+  prep.table = c.take<int4>(static_cast<size_t>(mx_max_chunks(max_rows, experts, prep.chunk_rows)) + 1);
+  prep.zero_out = zero_rest ? y : nullptr;
+  p.table = d.table = prep.table;
+  st = mx_prepare(x, act_dtype, max_rows, d_model, x_row_stride, xq, xs, prep, as_stream(stream));
+  if (st) return st;
+  p.x_codes = xq, p.x_scales = xs;
+  st = launch_mx_gemm(p, as_stream(stream));
+  return st ? st : launch_mx_gemm(d, as_stream(stream));
 }
 
 }  // extern "C"

@@ -1,27 +1,36 @@
 // Microscaled products of many rows on the scaled matrix instruction.
 //
-// One workgroup (8 waves) owns a row chunk (up to 32 * SUBT rows of one group)
-// and a tile of 256 stored weight rows: 256 columns of the result, or 128 gate
-// rows with the matching 128 up rows for 128 hidden columns.  Operands move
-// HBM/L2 -> LDS with global_load_lds in K slices of 256 columns (128 bytes of
-// codes, two matrix steps, and eight scale bytes per row) through a ring of two
-// or three stages, one barrier per slice, the next slices requested right after
-// it.  A load of codes is eight whole 128-byte row segments.  Every wave issues
-// the same loads per slice (rows past the end are clamped to a valid row, their
-// results never stored), so a fixed vmcnt marks a slice as landed.
+// The chip holds one workgroup (8 waves) per compute unit, each with a list of
+// tiles: a row chunk (up to 32 * SUBT rows of one group) by 256 stored weight
+// rows, 256 columns of the result, or 128 gate rows with the matching 128 up rows
+// for 128 hidden columns.  Operands move HBM/L2 -> LDS with global_load_lds in
+// slices of one matrix step (128 columns: 64 bytes of codes and four scale bytes
+// per row) through a ring of as many stages as the LDS holds (four at 320 rows,
+// seven at 64).  The ring runs on across tiles: while a tile's last slices are
+// multiplied and its result is stored, the first slices of the next are on their
+// way, so that neither a start nor an epilogue leaves the memory idle (one tile
+// per workgroup, whose slices of 256 columns began anew with each: 16384 rows of
+// 64 experts, d 2048, f 1024, gate and up 65 us, down 51 us, now @GATEUP@ and @DOWN@).
+// Every wave issues the same number of loads per slice (rows past the end are
+// clamped to a valid row, their results never stored; past the last slice the
+// last one is requested again), so a fixed vmcnt marks a slice as landed.
 //
-// LDS rows are 128 bytes; the eight 16-byte pieces of row r, each one block of 32
-// columns, are stored XOR-swizzled by (r >> 1) & 7, so the sixteen rows of a
-// fragment read hit distinct banks.  A lane's fragment of a step is one block
-// (piece 4 * step + lane / 16 of its row) and its scale byte.
+// LDS rows are 64 bytes, four 16-byte pieces, each one block of 32 columns; pieces
+// are stored XOR-swizzled so that the sixteen rows that a quarter wave reads cover
+// all banks.  Rows are stored ones in row order (gathered when they were
+// quantised), their scales step by step: dword [step][row].
 //
-// Waves form a 2 x 4 grid: wave (wm, wn) multiplies row sub-tiles wm, wm + 2, ...
-// (16 rows each) by its 64 weight rows; sub-tiles go in pairs, a pair past the
-// rows is not multiplied.  The weights are the instruction's first operand, so a
-// lane holds four consecutive columns of one row.  A wave's 32 hidden columns are
-// one block of the hidden row: its largest magnitude goes round the four lanes
-// that share the row, and silu(gate) * up leaves as codes, a quarter of the bytes
-// of a 16-bit row and nothing rounded on the way.
+// Waves form a 2 x 4 grid: wave (wm, wn) multiplies row tiles wm, wm + 2, ... (32
+// rows each) by its 64 weight rows, with the instruction of 32 x 32 rows and 64
+// columns (the 16 x 16 one issues twice the instructions for the same reads: 1743
+// against 1499 cycles a slice with every operand from LDS).  A lane's half h takes
+// blocks 2h and 2h + 1 of the slice, in the two steps, so one 16-bit read holds
+// both scales.  The weights are the instruction's first operand, so a lane holds
+// columns of one row; weight rows are dealt to the instruction's rows so that its
+// columns are consecutive: 32 of the result (whole 128-byte lines per row), or 16
+// hidden ones.  A wave's 32 hidden columns are one block of the hidden row: its
+// largest magnitude goes across the two lanes that share the row, and
+// silu(gate) * up leaves as codes, a quarter of the bytes of a 16-bit row.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -32,394 +41,439 @@ namespace qw {
 
 namespace {
 
-constexpr int MX_SLICE = 128;   // bytes of codes per row and slice: 256 columns
-constexpr int MX_SROW = 8;      // scale bytes per row and slice
-constexpr int MX_NB = 256;      // weight rows per workgroup
+constexpr int MX_ROWB = 64;     // bytes of codes per row and slice: 128 columns
+constexpr int MX_NB = 256;      // weight rows per tile
 constexpr int MX_THREADS = 512;
 constexpr int MX_WAVES = 8;
-constexpr int MX_NT = 4;        // 16-column tiles per wave
 constexpr int MX_LDS = 160 * 1024;
-constexpr int64_t kCus = 256;
+constexpr int kCus = 256;
 
 enum { MX_HIDDEN = -1 };        // epilogue: microscaled silu(gate) * up; else the output's dtype
 
-constexpr int mx_stage(int subt) { return (32 * subt + MX_NB) * (MX_SLICE + MX_SROW); }
-constexpr int mx_stages(int subt) { return MX_LDS / mx_stage(subt) >= 3 ? 3 : 2; }
+constexpr int mx_stage(int subt) { return (32 * subt + MX_NB) * (MX_ROWB + 4); }
+constexpr int mx_stages(int subt) { return MX_LDS / mx_stage(subt) < 8 ? MX_LDS / mx_stage(subt) : 8; }
 
-__device__ __forceinline__ int mx_swz(int row, int piece) { return piece ^ ((row >> 1) & 7); }
-
-// Workgroup -> tile.  Grouped rows (run > 0): the chunks that hold rows, found on
-// the device and dealt to the XCDs in runs that share their weights
-// (find_run_chunk), so that no bound on a group's rows can lose any.  One dense
-// group (run 0): the tiles in blocks of 8 row chunks by all columns, cut into one
-// contiguous part per XCD.
-struct MxGrid {
-  int n_tiles, run, row_chunks, per_xcd;
+struct MxTiles {
+  int n_tiles, row_chunks;  // row_chunks: of one dense group (chunk table NULL)
 };
 
 template <int EPI, int SUBT>
 __global__ __launch_bounds__(MX_THREADS) void mx_gemm_kernel(
-    const uint8_t* __restrict__ x_codes, const uint8_t* __restrict__ x_scales, const int32_t* __restrict__ row_index,
-    const int32_t* __restrict__ offsets, int max_rows, int groups, MxMatrix wa, MxMatrix wb, int n, int k_padded,
-    MxGrid grid, void* __restrict__ out, uint8_t* __restrict__ h_codes, uint8_t* __restrict__ h_scales) {
+    const uint8_t* __restrict__ x_codes, const uint8_t* __restrict__ x_scales, int rows,
+    const int4* __restrict__ table, MxMatrix wa, MxMatrix wb, int n, int k_padded, MxTiles grid,
+    void* __restrict__ out, bool wide, uint8_t* __restrict__ h_codes, uint8_t* __restrict__ h_scales) {
   constexpr bool GATEUP = EPI == MX_HIDDEN;
   constexpr int MCH = 32 * SUBT;
-  constexpr int A_STAGE = MCH * MX_SLICE, B_STAGE = MX_NB * MX_SLICE;
-  constexpr int AS_STAGE = MCH * MX_SROW, BS_STAGE = MX_NB * MX_SROW;
-  constexpr int STAGE = A_STAGE + B_STAGE + AS_STAGE + BS_STAGE;
-  constexpr int ST = mx_stages(SUBT), AHEAD = ST - 1;
-  constexpr int AG = MCH / 8, AL = (AG + MX_WAVES - 1) / MX_WAVES;  // 8-row load groups
-  constexpr int BL = MX_NB / 8 / MX_WAVES;
-  constexpr int ASL = (AS_STAGE / 256 + MX_WAVES - 1) / MX_WAVES;   // 256-byte scale loads
-  constexpr int BSL = BS_STAGE / 256 / MX_WAVES;
-  constexpr int LOADS = AL + BL + ASL + BSL;
-  static_assert(STAGE == mx_stage(SUBT) && ST * STAGE <= MX_LDS && AHEAD * LOADS < 64, "ring");
-  static_assert(AG % MX_WAVES == 0, "every wave loads the same number of groups");
+  constexpr int AG = MCH / 16, CG = AG + MX_NB / 16;       // 16-row load groups of codes: rows, then weights
+  constexpr int XG = MCH / 64, SG = XG + MX_NB / 64;       // 64-row load groups of scales
+  constexpr int CL = (CG + MX_WAVES - 1) / MX_WAVES, SL = (SG + MX_WAVES - 1) / MX_WAVES, LOADS = CL + SL;
+  constexpr int STAGE = mx_stage(SUBT), ST = mx_stages(SUBT), AHEAD = ST - 1;
+  constexpr int B_AT = AG * 1024, XS_AT = CG * 1024, WS_AT = XS_AT + XG * 256;
+  static_assert(SUBT % 2 == 0 && WS_AT + MX_NB * 4 == STAGE && AHEAD >= 2 && AHEAD * LOADS < 64, "ring");
+  static_assert(CG % 4 == 0 && CL * MX_WAVES - CG <= 4 && AG % 4 == 0, "groups per wave and their swizzles");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
-  // ---- tile of this workgroup ----
-  const int xcd = blockIdx.x % kXcds, j = blockIdx.x / kXcds;
-  int nt, mc = 0, e = 0;
-  int lo = 0, hi = max_rows;
-  if (grid.run == 0) {
-    const int t = xcd * grid.per_xcd + j;
-    if (t >= grid.n_tiles * grid.row_chunks) return;
-    const int block = 8 * grid.n_tiles, b0 = t / block * 8;
-    const int high = min(8, grid.row_chunks - b0);
-    const int r = t % block;
-    mc = b0 + r % high;
-    nt = r / high;
-  } else {
-    nt = j % grid.n_tiles;
-    e = find_run_chunk(offsets, groups, max_rows, MCH, grid.run, xcd, j / grid.n_tiles, &mc);
-    if (e < 0) return;
-    lo = max(offsets[e], 0);
-    hi = min(offsets[e + 1], max_rows);
-  }
-  const int r0 = lo + mc * MCH;
-  const int count = min(hi - r0, MCH);
-  if (count <= 0) return;
-
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int wm = wave / 4, wn = wave % 4;
-  const int l16 = lane % 16, lq = lane / 16;
-  const int n0 = nt * (GATEUP ? MX_NB / 2 : MX_NB);
   const uint32_t cb = k_padded / 2, sb = k_padded / kMxBlock;  // bytes of a row
-  const int KT = (k_padded + 255) / 256;
-  const bool half = k_padded % 256 != 0;  // the last slice holds one step
+  const int KT = k_padded / kMxStep;
 
-  // ---- sources of this wave's loads ----
-  // lane i of a code load writes LDS row 8g + i/8, physical piece i%8; g has the
-  // wave's parity in every load, so the logical piece is one per lane
-  const int piece = mx_swz(8 * (wave & 1) + lane / 8, lane % 8);
-  const int back = piece >= 4 ? -64 : 0;  // in a half slice the second step's pieces reread the first's
-  uint32_t a_src[AL];
-#pragma unroll
-  for (int q = 0; q < AL; ++q) {
-    const int row = 8 * (wave + q * MX_WAVES) + lane / 8;
-    const int rr = r0 + min(row, count - 1);
-    a_src[q] = static_cast<uint32_t>(row_index ? row_index[rr] : rr) * cb + piece * 16;
-  }
-  auto weight_row = [&](int row) {
-    return static_cast<uint32_t>(GATEUP ? min(n0 + row % (MX_NB / 2), n - 1) : min(n0 + row, n - 1));
+  // ---- this workgroup's tiles: one run of all tiles per XCD, dealt to its units ----
+  const int xcd = blockIdx.x % kXcds, unit = blockIdx.x / kXcds, units = gridDim.x / kXcds;
+  const int64_t all = static_cast<int64_t>(table ? table[0].x : grid.row_chunks) * grid.n_tiles;
+  const int first = static_cast<int>(all * xcd / kXcds), last = static_cast<int>(all * (xcd + 1) / kXcds);
+  struct Tile {
+    int e, r0, count, n0;
   };
-  // the weight rows of one load belong to one matrix: the first half of a wave's
-  // loads (GATEUP) reads gate, the second up
-  const uint8_t* const wa_c = wa.codes + static_cast<int64_t>(e) * n * cb;
-  const uint8_t* const wb_c = wb.codes + static_cast<int64_t>(e) * n * cb;
-  const uint8_t* const wa_s = wa.scales + static_cast<int64_t>(e) * n * sb;
-  const uint8_t* const wb_s = wb.scales + static_cast<int64_t>(e) * n * sb;
-  uint32_t b_src[BL];
+  auto tile_at = [&](int t) {
+    Tile r;
+    int nt;
+    if (table) {  // chunk by chunk: the tiles side by side share their rows
+      const int4 c = table[1 + t / grid.n_tiles];
+      nt = t % grid.n_tiles;
+      r.e = c.x, r.r0 = c.y, r.count = c.z;
+    } else {  // blocks of 8 row chunks by all columns
+      const int block = 8 * grid.n_tiles, b0 = t / block * 8;
+      const int high = min(8, grid.row_chunks - b0), q = t % block;
+      nt = q / high;
+      r.e = 0, r.r0 = (b0 + q % high) * MCH, r.count = min(rows - r.r0, MCH);
+    }
+    r.n0 = nt * (GATEUP ? MX_NB / 2 : MX_NB);
+    return r;
+  };
+  int at = first + unit;
+  if (at >= last) return;
+
+  // ---- loads ----
+  // Slot q of a wave is one load: of rows, or of weight rows (a wave-uniform fact).
+  const uint32_t lane_c = lane / 4 * cb, lane_s = lane * sb;
+  const uint32_t x_piece = ((lane % 4) ^ (lane / 16)) * 16;
+  const uint32_t w_piece = ((lane % 4) ^ (((GATEUP ? wave : wave >> 1) & 1) | (lane / 16 & 1) << 1)) * 16;
+  Tile req{0, 0, 0, 0};  // the tile whose slices are being requested; the first is set by the first advance
+  int req_kt = KT, req_at = at - units, stage = 0;
+  struct Slot {
+    int64_t base;              // address of the slice in the slot's first row
+    uint32_t row0, end;        // first row and last valid row, in bytes from there
+  };
+  Slot code_slot[CL], scale_slot[SL];
+  // group of a wave's load q (past the last group four back: another wave's group, the same swizzle)
+  auto code_group = [&](int q) {
+    const int g = wave + q * MX_WAVES;
+    return g >= CG ? g - 4 : g;
+  };
+  auto scale_group = [&](int q) { return min(wave + q * MX_WAVES, SG - 1); };
+  auto set_slots = [&] {
+    auto addr = [](const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); };
+    const int64_t w_row0 = static_cast<int64_t>(req.e) * n + req.n0;
+    const uint32_t x_end = req.count - 1, w_end = n - 1 - req.n0;
 #pragma unroll
-  for (int q = 0; q < BL; ++q)
-    b_src[q] = weight_row(8 * (wave + q * MX_WAVES) + lane / 8) * cb + piece * 16;
-  // a scale load is 64 dwords: 32 rows, the two steps' four bytes each
-  const int sback = lane % 2 ? -4 : 0;
-  uint32_t as_src[ASL];
-  int as_at[ASL];
+    for (int q = 0; q < CL; ++q) {
+      const int g = code_group(q), gw = g - AG;
+      const bool up = GATEUP && gw >= MX_NB / 32;
+      Slot& s = code_slot[q];
+      s.base = gw < 0 ? addr(x_codes) + static_cast<int64_t>(req.r0) * cb
+                      : addr(up ? wb.codes : wa.codes) + w_row0 * cb;
+      s.row0 = 16 * (gw < 0 ? g : up ? gw - MX_NB / 32 : gw) * cb;
+      s.end = (gw < 0 ? x_end : w_end) * cb;
+    }
 #pragma unroll
-  for (int q = 0; q < ASL; ++q) {
-    const int g = min(wave + q * MX_WAVES, AS_STAGE / 256 - 1);  // the last ones repeat a load
-    const int row = 32 * g + lane / 2;
-    const int rr = r0 + min(row, count - 1);
-    as_src[q] = static_cast<uint32_t>(row_index ? row_index[rr] : rr) * sb + lane % 2 * 4;
-    as_at[q] = g * 256;
-  }
-  const uint32_t bs_src = weight_row(32 * wave + lane / 2) * sb + lane % 2 * 4;
-  const uint8_t* const bs_base = GATEUP && __builtin_amdgcn_readfirstlane(wave) >= MX_WAVES / 2 ? wb_s : wa_s;
-  static_assert(BSL == 1, "one scale load of weight rows per wave");
-  auto issue = [&](int kt) {
-    char* const st = smem + (kt % ST) * STAGE;
-    const bool cut = half && kt == KT - 1;
-    const uint32_t off = kt * MX_SLICE + (cut ? back : 0), soff = kt * MX_SROW + (cut ? sback : 0);
+    for (int q = 0; q < SL; ++q) {
+      const int g = scale_group(q), gw = g - XG;
+      const bool up = GATEUP && gw >= MX_NB / 128;
+      Slot& s = scale_slot[q];
+      s.base = gw < 0 ? addr(x_scales) + static_cast<int64_t>(req.r0) * 4
+                      : addr(up ? wb.scales : wa.scales) + w_row0 * sb;
+      s.row0 = 64 * (gw < 0 ? g * 4 : (up ? gw - MX_NB / 128 : gw) * sb);
+      s.end = gw < 0 ? x_end * 4 : w_end * sb;
+    }
+  };
+  const int64_t xs_step = static_cast<int64_t>(rows) * 4;  // from step to step of the rows' scales
+  auto request = [&] {
+    char* const st = smem + stage;
 #pragma unroll
-    for (int q = 0; q < AL; ++q)
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(x_codes + (a_src[q] + off)),
-                                       (lds_void*)(st + (wave + q * MX_WAVES) * 1024), 16, 0, 0);
+    for (int q = 0; q < CL; ++q) {
+      const int g = code_group(q);
+      Slot& s = code_slot[q];
+      const uint32_t off = min(s.row0 + lane_c, s.end) + (g < AG ? x_piece : w_piece);
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint8_t*>(static_cast<uintptr_t>(s.base)) + off,
+                                       (lds_void*)(st + g * 1024), 16, 0, 0);
+      s.base += MX_ROWB;
+    }
 #pragma unroll
-    for (int q = 0; q < BL; ++q)
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>((GATEUP && q >= BL / 2 ? wb_c : wa_c) + (b_src[q] + off)),
-                                       (lds_void*)(st + A_STAGE + (wave + q * MX_WAVES) * 1024), 16, 0, 0);
-#pragma unroll
-    for (int q = 0; q < ASL; ++q)
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(x_scales + (as_src[q] + soff)),
-                                       (lds_void*)(st + A_STAGE + B_STAGE + as_at[q]), 4, 0, 0);
-    __builtin_amdgcn_global_load_lds(static_cast<const void*>(bs_base + (bs_src + soff)),
-                                     (lds_void*)(st + A_STAGE + B_STAGE + AS_STAGE + wave * 256), 4, 0, 0);
+    for (int q = 0; q < SL; ++q) {
+      const int g = scale_group(q);
+      Slot& s = scale_slot[q];
+      const uint32_t off = min(s.row0 + (g < XG ? lane * 4u : lane_s), s.end);
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint8_t*>(static_cast<uintptr_t>(s.base)) + off,
+                                       (lds_void*)(st + XS_AT + g * 256), 4, 0, 0);
+      s.base += g < XG ? xs_step : 4;
+    }
+    stage = stage + STAGE == ST * STAGE ? 0 : stage + STAGE;
+    ++req_kt;
+  };
+  // Before a request, where the tile's slices are all requested: the next tile.
+  auto advance = [&] {
+    if (req_kt < KT) return;
+    if (req_at + units < last) {
+      req_at += units;
+      req = tile_at(req_at);
+    }  // else nothing is left: the last tile's slices again, into stages that are not read
+    req_kt = 0;
+    set_slots();
   };
 
-  f32x4 acc[SUBT][MX_NT];
-#pragma unroll
-  for (int i = 0; i < SUBT; ++i)
-#pragma unroll
-    for (int t = 0; t < MX_NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // this lane's fragment in a stage: its row of sub-tile wm, of weight tile 0, and their scales
-  const int frag = l16 * MX_SLICE + mx_swz(l16, lq) * 16;
-  const int b_row = wn * (GATEUP ? 32 : 64);
-  const int a_lane = wm * 16 * MX_SLICE + frag, b_lane = b_row * MX_SLICE + frag;
-  const int as_lane = (wm * 16 + l16) * MX_SROW + lq, bs_lane = (b_row + l16) * MX_SROW + lq;
-  const int active_sub = (count + 15) / 16;
-
-  for (int s = 0; s < AHEAD && s < KT; ++s) issue(s);
-
-  // One slice: STEPS matrix steps for NPA pairs of sub-tiles.  Fragments of the
-  // next unit (a step of a pair) are read right after the first instruction of
-  // the current one.
-  struct Frag {
-    u32x4 v;
-    uint32_t s;
+  // ---- fragments: one address per operand, the rest are constant offsets ----
+  const int l32 = lane % 32, half = lane / 32;
+  // instruction row 8j + 4h + c is weight row 4j + c of the lane half h's run
+  const int w_run = (l32 >> 3) * 4 + (l32 & 3), w_half = l32 >> 2 & 1;
+  const int w_row = GATEUP ? wn * 32 + w_half * 16 + w_run : wn * 64 + w_half * 32 + w_run;
+  constexpr int W_TILE = GATEUP ? MX_NB / 2 : 16;  // from weight tile to weight tile: up's rows, or the run's other half
+  const int a_lane = (wm * 32 + l32) * MX_ROWB + (((2 * half) ^ (l32 >> 2 & 3)) * 16);
+  const int b_lane = B_AT + w_row * MX_ROWB + (((2 * half) ^ (w_half | (l32 >> 3 & 1) << 1)) * 16);
+  const int as_lane = XS_AT + (wm * 32 + l32) * 4 + 2 * half, bs_lane = WS_AT + w_row * 4 + 2 * half;
+  auto read_a = [&](const char* st, int i, int step) {
+    return *reinterpret_cast<const u32x4*>(st + (a_lane ^ (step * 16)) + i * 64 * MX_ROWB);
   };
-  auto slice = [&](auto npa, auto steps, const char* st, auto&& request) {
-    constexpr int NPA = decltype(npa)::value, STEPS = decltype(steps)::value;
-    // one address per step and operand, the rest are constant offsets: a row's swizzle
-    // is that of its lane, and the second step's pieces lie 64 bytes across
-    const char* const a0 = st + a_lane;
-    const char* const a1 = st + (a_lane ^ 64);
-    const char* const b0 = st + A_STAGE + b_lane;
-    const char* const b1 = st + A_STAGE + (b_lane ^ 64);
-    const char* const as = st + A_STAGE + B_STAGE + as_lane;
-    const char* const bs = st + A_STAGE + B_STAGE + AS_STAGE + bs_lane;
-    auto read_a = [&](int i, int ks) {
-      Frag f;
-      f.v = *reinterpret_cast<const u32x4*>((ks ? a1 : a0) + i * 32 * MX_SLICE);
-      f.s = *reinterpret_cast<const uint8_t*>(as + i * 32 * MX_SROW + ks * 4);
-      return f;
-    };
-    auto read_b = [&](int t, int ks) {
-      const int row = GATEUP ? t / 2 * (MX_NB / 2) + t % 2 * 16 : t * 16;
-      Frag f;
-      f.v = *reinterpret_cast<const u32x4*>((ks ? b1 : b0) + row * MX_SLICE);
-      f.s = *reinterpret_cast<const uint8_t*>(bs + row * MX_SROW + ks * 4);
-      return f;
-    };
-    Frag w[2][MX_NT], xb[2][2];
+  auto read_as = [&](const char* st, int i) {
+    return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(st + as_lane + i * 64 * 4));
+  };
+  auto read_b = [&](const char* st, int t, int step) {
+    return *reinterpret_cast<const u32x4*>(st + (b_lane ^ (step * 16)) + t * W_TILE * MX_ROWB);
+  };
+  auto read_bs = [&](const char* st, int t) {
+    return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(st + bs_lane + t * W_TILE * 4));
+  };
+  constexpr int NT = SUBT / 2;  // row tiles of a wave
+  f32x16 acc[NT][2];
+
+  // Fragments are read two units (a row tile in a step) ahead of their
+  // instructions, across slices too: a slice starts with its first step's weight
+  // fragments, both steps' weight scales and its first two units in registers.
+  u32x4 w[2], x[2];
+  uint32_t ws[2], xs[2];
+  auto read_first = [&](const char* st, auto npa) {
+    constexpr int NPA = decltype(npa)::value;
 #pragma unroll
-    for (int t = 0; t < MX_NT; ++t) w[0][t] = read_b(t, 0);
-    xb[0][0] = read_a(0, 0);
-    xb[0][1] = read_a(1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * MX_NT + 4, 0);
+    for (int t = 0; t < 2; ++t) w[t] = read_b(st, t, 0), ws[t] = read_bs(st, t);
+    x[0] = read_a(st, 0, 0), xs[0] = read_as(st, 0);
+    x[1] = read_a(st, 1 % NPA, 1 / NPA), xs[1] = read_as(st, 1 % NPA);
+  };
+  auto slice = [&](auto npa, const char* st, const char* next) {
+    constexpr int NPA = decltype(npa)::value, UNITS = 2 * NPA;
+    u32x4 xq[UNITS + 2], w1[2], wn[2];
+    uint32_t sq[UNITS + 2], wsn[2];  // the scale of a unit; both steps of a tile share it
+    xq[0] = x[0], xq[1] = x[1], sq[0] = xs[0], sq[1] = xs[1];
     request();
 #pragma unroll
-    for (int u = 0; u < STEPS * NPA; ++u) {
-      const int ks = u / NPA, p = u % NPA;
-      const Frag x0 = xb[u & 1][0], x1 = xb[u & 1][1];
-      acc[2 * p][0] = mx_mfma(w[ks][0].v, x0.v, acc[2 * p][0], w[ks][0].s, x0.s);
+    for (int u = 0; u < UNITS; ++u) {
+      const int i = u % NPA;
+      auto multiply = [&](int t) {
+        if (u < NPA) acc[i][t] = mx_mfma32<0>(w[t], xq[u], acc[i][t], ws[t], sq[u]);
+        else acc[i][t] = mx_mfma32<1>(w1[t], xq[u], acc[i][t], ws[t], sq[u]);
+      };
+      multiply(0);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (u + 1 < STEPS * NPA) {
-        const int ks1 = (u + 1) / NPA, p1 = (u + 1) % NPA;
-        if (ks1 != ks) {
-#pragma unroll
-          for (int t = 0; t < MX_NT; ++t) w[ks1][t] = read_b(t, ks1);
-          xb[(u + 1) & 1][0] = read_a(2 * p1, ks1);
-          xb[(u + 1) & 1][1] = read_a(2 * p1 + 1, ks1);
-          __builtin_amdgcn_sched_group_barrier(0x100, 2 * MX_NT + 4, 0);
-        } else {
-          xb[(u + 1) & 1][0] = read_a(2 * p1, ks1);
-          xb[(u + 1) & 1][1] = read_a(2 * p1 + 1, ks1);
-          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-        }
+      // two units ahead
+      const int v = u + 2 < UNITS ? u + 2 : u + 2 - UNITS;
+      xq[u + 2] = read_a(u + 2 < UNITS ? st : next, v % NPA, v / NPA);
+      if (u + 2 < UNITS && v >= NPA) {
+        sq[u + 2] = sq[v - NPA];
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      } else {
+        sq[u + 2] = read_as(u + 2 < UNITS ? st : next, v % NPA);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       }
-#pragma unroll
-      for (int t = 1; t < MX_NT; ++t) acc[2 * p][t] = mx_mfma(w[ks][t].v, x0.v, acc[2 * p][t], w[ks][t].s, x0.s);
-#pragma unroll
-      for (int t = 0; t < MX_NT; ++t)
-        acc[2 * p + 1][t] = mx_mfma(w[ks][t].v, x1.v, acc[2 * p + 1][t], w[ks][t].s, x1.s);
-      __builtin_amdgcn_sched_group_barrier(0x008, 2 * MX_NT - 1, 0);
+      if (u == 0) {  // the second step's weights
+        w1[0] = read_b(st, 0, 1), w1[1] = read_b(st, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      if (u == NPA) {  // the next slice's
+        wn[0] = read_b(next, 0, 0), wn[1] = read_b(next, 1, 0);
+        wsn[0] = read_bs(next, 0), wsn[1] = read_bs(next, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      }
+      multiply(1);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
+    x[0] = xq[UNITS], x[1] = xq[UNITS + 1], xs[0] = sq[UNITS], xs[1] = sq[UNITS + 1];
+    w[0] = wn[0], w[1] = wn[1], ws[0] = wsn[0], ws[1] = wsn[1];
   };
-  constexpr int NP = SUBT / 2;
-  static_assert(SUBT % 2 == 0 && AHEAD >= 1 && AHEAD <= 2, "pairs; ring depth");
-  auto k_loop = [&](auto npa) {
-    using Two = std::integral_constant<int, 2>;
-    using One = std::integral_constant<int, 1>;
-    // slice kt has landed when only the slices requested after it may be in flight
-    int kt = 0;
-    for (; kt < KT - AHEAD; ++kt) {
-      wait_vmcnt<(AHEAD - 1) * LOADS>();
-      ring_barrier();
-      slice(npa, Two{}, smem + (kt % ST) * STAGE, [&] { issue(kt + AHEAD); });
-    }
-    for (const int full = half ? KT - 1 : KT; kt < full; ++kt) {
-      if (AHEAD == 2 && kt + 1 < KT) wait_vmcnt<LOADS>();
-      else wait_vmcnt<0>();
-      ring_barrier();
-      slice(npa, Two{}, smem + (kt % ST) * STAGE, [] {});
-    }
-    if (half) {
-      wait_vmcnt<0>();
-      ring_barrier();
-      slice(npa, One{}, smem + (kt % ST) * STAGE, [] {});
-    }
-  };
-  const int wave_sub = active_sub > wm ? (active_sub - wm + 1) / 2 : 0;
-  const int npa = __builtin_amdgcn_readfirstlane((wave_sub + 1) / 2);
-  if constexpr (NP >= 4) {
-    if (npa >= NP) k_loop(std::integral_constant<int, NP>{});
-    else if (npa >= 3) k_loop(std::integral_constant<int, (NP > 4 ? 4 : 3)>{});
-    else k_loop(std::integral_constant<int, 2>{});
-  } else {
-    k_loop(std::integral_constant<int, NP>{});
-  }
 
-  // ---- epilogue: lane holds row l16 of a sub-tile, columns 4 lq .. 4 lq + 3 of each tile ----
-  if constexpr (GATEUP) {
-    const int64_t np = (n + kMxStep - 1) / kMxStep * static_cast<int64_t>(kMxStep);
-    const int c0 = n0 + wn * 32 + 4 * lq;
+#pragma unroll 1
+  for (int s = 0; s < AHEAD; ++s) {
+    advance();
+    request();
+  }
+  wait_vmcnt<LOADS>();  // all but the newest slice
+  ring_barrier();
+  int read_at = 0;  // the stage that is multiplied
+  Tile tile = tile_at(at);
+  for (; at < last; at += units) {
 #pragma unroll
-    for (int i = 0; i < SUBT; ++i) {
-      const int s = wm + 2 * i;
-      if (s >= active_sub) continue;  // wave-uniform
-      const int row = s * 16 + l16;
-      float h[2][4];
-      uint32_t top = 0;
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          // padding columns of the hidden row are zero codes
-          h[t][q] = c0 + t * 16 + q < n ? mx_swiglu(acc[i][t][q], acc[i][t + 2][q]) : 0.0f;
-          top = max(top, __float_as_uint(h[t][q]) & 0x7fffffffu);
-        }
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, kWave)));
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, kWave)));
-      const uint32_t sc = mx_scale_of(top);
-      const float div = mx_divisor(sc);
-      uint32_t code[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        code[t] = mx_pack_f32<0>(0u, h[t][0], h[t][1], div);
-        code[t] = sc == kMxNan ? 0u : mx_pack_f32<1>(code[t], h[t][2], h[t][3], div);
+        for (int q = 0; q < 16; ++q) acc[i][t][q] = 0.f;
+    const int tiles = __builtin_amdgcn_readfirstlane((tile.count + 31) / 32);  // row tiles holding valid rows
+    auto k_loop = [&](auto npa) {
+      read_first(smem + read_at, npa);
+      for (int kt = 0; kt < KT; ++kt) {
+        // the slice after this one has landed (a tile's first slices were waited for
+        // before the stores of the tile before it) ...
+        if (kt >= AHEAD - 2) wait_vmcnt<(AHEAD - 2) * LOADS>();
+        ring_barrier();  // ... for every wave, and every wave is done with the slice before this one
+        advance();       // ahead of the slice: its matrix instructions stay with its reads in one block
+        const int next = read_at + STAGE == ST * STAGE ? 0 : read_at + STAGE;
+        slice(npa, smem + read_at, smem + next);
+        read_at = next;
       }
-      if (row < count) {
-        uint8_t* const o = h_codes + (r0 + row) * (np / 2) + c0 / 2;
-        *reinterpret_cast<uint16_t*>(o) = static_cast<uint16_t>(code[0]);
-        *reinterpret_cast<uint16_t*>(o + 8) = static_cast<uint16_t>(code[1]);
-        if (lq == 0) h_scales[(r0 + row) * (np / kMxBlock) + c0 / kMxBlock] = static_cast<uint8_t>(sc);
-      }
+    };
+    // a wave's row tiles wm, wm + 2, ... below `tiles` hold rows
+    const int mine = tiles > wm ? (tiles - wm + 1) / 2 : 0;
+    if constexpr (NT >= 2) {
+      if (mine > (NT + 1) / 2) k_loop(std::integral_constant<int, NT>{});
+      else k_loop(std::integral_constant<int, (NT + 1) / 2>{});
+    } else {
+      k_loop(std::integral_constant<int, NT>{});
     }
-  } else {
-    const bool vec = n % 4 == 0;
+    const Tile done = tile;
+    if (at + units < last) tile = tile_at(at + units);
+    // the slices requested so far but the newest, before the stores go into the same queue
+    wait_vmcnt<LOADS>();
+
+    // ---- epilogue: lane holds row l32 of a tile ----
+    const int r0 = done.r0;
+    if constexpr (GATEUP) {
+      const int64_t np = (n + kMxStep - 1) / kMxStep * static_cast<int64_t>(kMxStep);
+      const int c0 = done.n0 + wn * 32 + 16 * half;
+      uint8_t* const hs = h_scales + (static_cast<int64_t>(done.n0 / kMxStep) * rows + r0) * 4 + wn;
 #pragma unroll
-    for (int i = 0; i < SUBT; ++i) {
-      const int s = wm + 2 * i;
-      if (s >= active_sub) continue;
-      const int row = s * 16 + l16;
-      if (row >= count) continue;
-      const int64_t orow = static_cast<int64_t>(r0 + row) * n;
+      for (int i = 0; i < NT; ++i) {
+        if (wm + 2 * i >= tiles) continue;  // wave-uniform
+        const int row = (wm + 2 * i) * 32 + l32;
+        float h[16];
+        uint32_t top = 0;
 #pragma unroll
-      for (int t = 0; t < MX_NT; ++t) {
-        const int col = n0 + wn * 64 + t * 16 + 4 * lq;
-        const float v[4] = {acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
-        if (vec && col < n) {
-          store_vec<EPI, 4>(out, orow + col, v);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (col + q < n) store_act<EPI>(out, orow + col + q, v[q]);
+        for (int q = 0; q < 16; ++q) {
+          // padding columns of the hidden row are zero codes
+          h[q] = c0 + q < n ? mx_swiglu(acc[i][0][q], acc[i][1][q]) : 0.0f;
+          top = max(top, __float_as_uint(h[q]) & 0x7fffffffu);
         }
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, kWave)));
+        const uint32_t sc = mx_scale_of(top);
+        const float div = mx_divisor(sc);
+        uint32_t code[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          code[q] = mx_pack_f32<0>(0u, h[8 * q], h[8 * q + 1], div);
+          code[q] = mx_pack_f32<1>(code[q], h[8 * q + 2], h[8 * q + 3], div);
+          code[q] = mx_pack_f32<2>(code[q], h[8 * q + 4], h[8 * q + 5], div);
+          code[q] = mx_pack_f32<3>(code[q], h[8 * q + 6], h[8 * q + 7], div);
+          if (sc == kMxNan) code[q] = 0u;
+        }
+        if (row < done.count) {
+          *reinterpret_cast<uint2*>(h_codes + (r0 + row) * (np / 2) + c0 / 2) = make_uint2(code[0], code[1]);
+          if (half == 0) hs[row * 4] = static_cast<uint8_t>(sc);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // tile by tile: the accumulators leave no registers for two
+      }
+    } else {
+      // 16-bit results go through LDS, a row tile at a time in this wave's part of the
+      // stage that the next request will fill (free once every wave is done with the
+      // last slice), so that a store is eight whole 128-byte lines (a lane's own 16
+      // bytes of 32 rows each: 320 x 256 results 12 us instead of @EPI@).
+      constexpr int PASSES = MX_WAVES * 32 * 128 <= STAGE ? 1 : 2;  // sixteen rows at a time in small stages
+      constexpr int MINE = 32 * 128 / PASSES;
+      static_assert(MX_WAVES * MINE <= STAGE, "the rows of every wave fit a stage");
+      const int free_at = read_at == 0 ? (ST - 1) * STAGE : read_at - STAGE;
+      char* const st = smem + free_at + wave * MINE;
+      if (EPI != QW_F32 && wide) ring_barrier();
+      const int col = done.n0 + wn * 64;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        if (wm + 2 * i >= tiles) continue;
+        const int row0 = (wm + 2 * i) * 32;
+        if (EPI != QW_F32 && wide) {
+          // 16-byte chunk c of row r at chunk c ^ (r & 7): a lane writes chunks of one row, reads one of eight rows
+          const int c = lane % 8;
+#pragma unroll
+          for (int pass = 0; pass < PASSES; ++pass) {
+            constexpr int R = 32 / PASSES;
+            if (PASSES == 1 || l32 / R == pass) {
+#pragma unroll
+              for (int q = 0; q < 32; q += 8) {
+                u32x4 v;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  v[k] = pack_half2<EPI == QW_F16 ? QW_F16 : QW_BF16>(acc[i][q / 16][q % 16 + 2 * k],
+                                                                      acc[i][q / 16][q % 16 + 2 * k + 1]);
+                *reinterpret_cast<u32x4*>(st + l32 % R * 128 + (((half * 4 + q / 8) ^ (l32 & 7)) * 16)) = v;
+              }
+            }
+            wave_lds_order();
+            u32x4 v[R / 8];
+#pragma unroll
+            for (int q = 0; q < R / 8; ++q) {
+              const int r = q * 8 + lane / 8;
+              v[q] = *reinterpret_cast<const u32x4*>(st + r * 128 + ((c ^ (r & 7)) * 16));
+            }
+            wave_lds_order();
+#pragma unroll
+            for (int q = 0; q < R / 8; ++q) {
+              const int row = row0 + pass * R + q * 8 + lane / 8;
+              if (row < done.count && col + c * 8 < n)
+                *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + static_cast<int64_t>(r0 + row) * n + col +
+                                          c * 8) = v[q];
+            }
+          }
+        } else {
+          const int row = row0 + l32, c0 = col + half * 32;
+          if (row >= done.count) continue;
+          const int64_t o = static_cast<int64_t>(r0 + row) * n + c0;
+          if (wide && c0 + 32 <= n) {  // fp32
+#pragma unroll
+            for (int q = 0; q < 32; q += 4) {
+              const float v[4] = {acc[i][q / 16][q % 16], acc[i][q / 16][q % 16 + 1], acc[i][q / 16][q % 16 + 2],
+                                  acc[i][q / 16][q % 16 + 3]};
+              store_vec<QW_F32, 4>(out, o + q, v);
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+              if (c0 + q < n) store_act<EPI>(out, o + q, acc[i][q / 16][q % 16]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
+  wait_vmcnt<0>();  // the LDS is not given back while requests for it are on their way
 }
 
 template <int EPI, int SUBT>
 int launch_t(const MxProduct& p, hipStream_t stream) {
-  constexpr int MCH = 32 * SUBT;
-  constexpr bool GATEUP = EPI == MX_HIDDEN;
-  MxGrid g;
-  g.n_tiles = static_cast<int>(GATEUP ? ceil_div(p.n, MX_NB / 2) : ceil_div(p.n, MX_NB));
-  g.row_chunks = static_cast<int>(ceil_div(p.rows, MCH));
-  g.per_xcd = g.run = 0;
-  int64_t chunks;
-  if (p.offsets == nullptr) {
-    const int64_t tiles = static_cast<int64_t>(g.n_tiles) * g.row_chunks;
-    if (tiles > INT32_MAX / 16) return set_error(QW_ERR_UNSUPPORTED, "too many tiles for one microscaled product");
-    g.per_xcd = static_cast<int>(ceil_div(tiles, kXcds));
-    chunks = g.per_xcd;
-  } else {
-    const int run = loose_run(p.rows, p.groups, MCH);
-    g.run = run;
-    chunks = loose_chunks(p.rows, p.groups, MCH, run) * g.n_tiles;
-  }
-  const int64_t blocks = kXcds * chunks;
-  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many tiles for one microscaled product");
+  MxTiles g;
+  g.n_tiles = static_cast<int>(EPI == MX_HIDDEN ? ceil_div(p.n, MX_NB / 2) : ceil_div(p.n, MX_NB));
+  g.row_chunks = static_cast<int>(ceil_div(p.rows, 32 * SUBT));
+  const int64_t chunks = p.table ? g.row_chunks + p.groups : g.row_chunks;
+  if (chunks * g.n_tiles > INT32_MAX / 16)
+    return set_error(QW_ERR_UNSUPPORTED, "too many tiles for one microscaled product");
+  const int64_t units = std::min<int64_t>(kCus / kXcds, ceil_div(chunks * g.n_tiles, kXcds));
   constexpr int lds = mx_stages(SUBT) * mx_stage(SUBT);
   const hipError_t attr = reserve_lds<mx_gemm_kernel<EPI, SUBT>>(lds);
   if (attr != hipSuccess)
     return set_error(QW_ERR_HIP, "cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(attr));
-  mx_gemm_kernel<EPI, SUBT><<<static_cast<unsigned>(blocks), MX_THREADS, lds, stream>>>(
-      p.x_codes, p.x_scales, p.row_index, p.offsets, static_cast<int>(p.rows), static_cast<int>(p.groups), p.a, p.b,
-      static_cast<int>(p.n), static_cast<int>(mx_padded(p.k)), g, p.out, p.h_codes, p.h_scales);
+  const int size = EPI == QW_F32 ? 4 : 2;
+  const bool wide = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.n * size % 16 == 0;
+  mx_gemm_kernel<EPI, SUBT><<<static_cast<unsigned>(units * kXcds), MX_THREADS, lds, stream>>>(
+      p.x_codes, p.x_scales, static_cast<int>(p.rows), p.table, p.a, p.b, static_cast<int>(p.n),
+      static_cast<int>(mx_padded(p.k)), g, p.out, wide, p.h_codes, p.h_scales);
   QW_LAUNCH_CHECK("mx_gemm_kernel");
   return QW_OK;
 }
 
 template <int EPI>
-int launch_sel(int subt, const MxProduct& p, hipStream_t stream) {
-  switch (subt) {
-    case 2: return launch_t<EPI, 2>(p, stream);
-    case 4: return launch_t<EPI, 4>(p, stream);
-    case 6: return launch_t<EPI, 6>(p, stream);
-    case 8: return launch_t<EPI, 8>(p, stream);
+int launch_sel(const MxProduct& p, hipStream_t stream) {
+  switch (p.chunk_rows) {
+    case 64: return launch_t<EPI, 2>(p, stream);
+    case 128: return launch_t<EPI, 4>(p, stream);
+    case 192: return launch_t<EPI, 6>(p, stream);
+    case 256: return launch_t<EPI, 8>(p, stream);
     default: return launch_t<EPI, 10>(p, stream);
   }
 }
 
-// Sub-tile pairs of a workgroup.  Dense rows: the chunk height whose tiles cost
-// the fewest rounds of the chip.  Grouped rows: the smallest chunk that holds the
-// usual group (even routing and 3.5 standard deviations, within the bound).
-int pick_subt(const MxProduct& p, bool gateup) {
-  const int64_t n_tiles = gateup ? ceil_div(p.n, MX_NB / 2) : ceil_div(p.n, MX_NB);
-  if (p.offsets == nullptr) {
-    int best = 2;
-    int64_t cost = INT64_MAX;
-    for (int s : {2, 4, 6, 8, 10}) {
-      // a tile costs its rows and its weight rows' loads
-      const int64_t c = ceil_div(ceil_div(p.rows, 32 * s) * n_tiles, kCus) * (32 * s + 96);
-      if (c <= cost) best = s, cost = c;
-    }
-    return best;
-  }
-  const int64_t avg = std::min(p.row_cap, ceil_div(p.rows, p.groups));
-  const int64_t likely = std::min(p.row_cap, avg + static_cast<int64_t>(3.5 * std::sqrt(static_cast<double>(avg))));
-  const int64_t rows = p.row_cap <= 320 && p.row_cap <= 2 * avg ? p.row_cap : likely;
-  for (int s : {2, 4, 6, 8})
-    if (rows <= 32 * s) return s;
-  return 10;
-}
-
 }  // namespace
 
+// Dense rows: the chunk height whose tiles cost the fewest rounds of the chip (a
+// tile costs its rows and the loads of its weight rows).
+int mx_dense_chunk(int64_t rows, int64_t n) {
+  int best = 64;
+  int64_t cost = INT64_MAX;
+  for (int h : {64, 128, 192, 256, 320}) {
+    const int64_t c = ceil_div(ceil_div(rows, h) * ceil_div(n, MX_NB), kCus) * (h + 96);
+    if (c <= cost) best = h, cost = c;
+  }
+  return best;
+}
+
+// Grouped rows: the smallest chunk that holds the usual group (even routing and
+// 3.5 standard deviations, within the bound).
+int mx_group_chunk(int64_t rows, int64_t groups, int64_t cap) {
+  const int64_t avg = std::min(cap, ceil_div(rows, groups));
+  const int64_t likely = std::min(cap, avg + static_cast<int64_t>(3.5 * std::sqrt(static_cast<double>(avg))));
+  const int64_t want = cap <= 320 && cap <= 2 * avg ? cap : likely;
+  for (int h : {64, 128, 192, 256})
+    if (want <= h) return h;
+  return 320;
+}
+
 int launch_mx_gemm(const MxProduct& p, hipStream_t stream) {
-  const bool gateup = p.h_codes != nullptr;
-  // rows are addressed by 32-bit offsets from the matrix (or the rows') start
-  if (std::max(p.rows, p.x_rows) * mx_code_bytes(p.k) > UINT32_MAX || p.n * mx_code_bytes(p.k) > UINT32_MAX)
-    return launch_mx_rows(p, stream);
-  const int subt = pick_subt(p, gateup);
-  if (gateup) return launch_sel<MX_HIDDEN>(subt, p, stream);
-  if (p.out_dtype == QW_F32) return launch_sel<QW_F32>(subt, p, stream);
-  if (p.out_dtype == QW_F16) return launch_sel<QW_F16>(subt, p, stream);
-  return launch_sel<QW_BF16>(subt, p, stream);
+  if (p.h_codes) return launch_sel<MX_HIDDEN>(p, stream);
+  if (p.out_dtype == QW_F32) return launch_sel<QW_F32>(p, stream);
+  if (p.out_dtype == QW_F16) return launch_sel<QW_F16>(p, stream);
+  return launch_sel<QW_BF16>(p, stream);
 }
 
 }  // namespace qw

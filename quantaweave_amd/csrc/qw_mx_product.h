@@ -12,12 +12,16 @@ struct MxMatrix {
 };
 
 // Rows times matrices.  Rows are grouped by `offsets` (device, groups + 1; NULL:
-// one group holding all `rows`).  The rows are stored ones (x_codes, x_scales) or
-// numbers of x_dtype (x, x_stride), quantised on the way; row_index picks the
-// row behind each (NULL: the row itself).
+// one group holding all `rows`).
 //   one matrix  : out[r] = x[r] . a[n]               [rows, n] of out_dtype
 //   two matrices: h[r] = silu(x[r] . a[n]) * (x[r] . b[n]), stored microscaled:
-//                 h_codes [rows, padded(n) / 2], h_scales [rows, padded(n) / 32]
+//                 h_codes [rows, padded(n) / 2] and h_scales
+// launch_mx_rows takes numbers of x_dtype (x, x_stride; row_index picks the row
+// behind each, NULL: the row itself) or stored rows (x_codes, x_scales), with the
+// scales of stored rows and of h as [rows][padded / 32].
+// launch_mx_gemm takes stored rows in row order, with the scales of rows and of h
+// step by step, [padded / 128][rows][4], and grouped rows as a chunk table:
+// table[0].x chunks, table[1 + i] = {group, first row, rows, 0} of up to chunk_rows.
 struct MxProduct {
   const void* x = nullptr;
   int x_dtype = QW_F32;
@@ -26,10 +30,13 @@ struct MxProduct {
   const uint8_t* x_scales = nullptr;
   const int32_t* row_index = nullptr;
   const int32_t* offsets = nullptr;
-  int64_t groups = 1, rows = 0, x_rows = 0, row_cap = 0, n = 0, k = 0;  // x_rows: rows behind row_index
+  const int4* table = nullptr;
+  int chunk_rows = 0;
+  int64_t groups = 1, rows = 0, n = 0, k = 0;
   MxMatrix a{nullptr, nullptr}, b{nullptr, nullptr};
   void* out = nullptr;
   int out_dtype = QW_F32;
+  bool zero_rest = false;  // launch_mx_rows: rows of no group become zeros
   uint8_t* h_codes = nullptr;
   uint8_t* h_scales = nullptr;
 };
@@ -38,9 +45,26 @@ struct MxProduct {
 int launch_mx_rows(const MxProduct& p, hipStream_t stream);
 // Many rows (stored ones): tiles of the matrix instruction through LDS.
 int launch_mx_gemm(const MxProduct& p, hipStream_t stream);
+// Row chunks of launch_mx_gemm: one dense group, and grouped rows with a bound on a group's.
+int mx_dense_chunk(int64_t rows, int64_t n);
+int mx_group_chunk(int64_t rows, int64_t groups, int64_t cap);
+// Most chunks that `rows` rows in `groups` groups make, and the bytes of their table.
+inline int64_t mx_max_chunks(int64_t rows, int64_t groups, int chunk) { return ceil_div(rows, chunk) + groups; }
 
 // Whether a product of `rows` rows in `groups` groups is one of few rows.
 inline bool mx_few_rows(int64_t rows, int64_t groups) { return rows <= groups * 16; }
+
+// What launch_mx_gemm's rows need beside quantisation, in the same pass.
+struct MxPrepare {
+  const int32_t* row_index = nullptr;  // gather
+  const int32_t* offsets = nullptr;    // grouped rows: the chunk table
+  int64_t groups = 0;
+  int4* table = nullptr;
+  int chunk_rows = 0;
+  void* zero_out = nullptr;            // rows of no group become zeros here ([rows, cols] of x's type)
+};
+int mx_prepare(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, uint8_t* codes, uint8_t* scales,
+               const MxPrepare& prep, hipStream_t stream);
 
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
                 hipStream_t stream);

@@ -20,11 +20,33 @@ constexpr int kRowsWaves = 8, kRowsThreads = kRowsWaves * kWave;
 constexpr int kRowsM = 16, kRowsN = 32;
 constexpr int kStored = -1;  // XDT of rows that are stored microscaled
 
+// The workgroups past the groups' last tile: zeros in the rows behind the last
+// group, sixteen rows by 32 columns each.
+__device__ void zero_rows(const int32_t* __restrict__ offsets, int groups, int rows, int chunk, int ct, int n,
+                          void* __restrict__ out, int out_dtype) {
+  const int lane = threadIdx.x % kWave;
+  int tiles = 0;
+  for (int e0 = 0; e0 < groups; e0 += kWave) {
+    int c = 0;
+    if (e0 + lane < groups) {
+      const int lo = min(max(offsets[e0 + lane], 0), rows), hi = min(offsets[e0 + lane + 1], rows);
+      c = hi > lo ? (hi - lo + kRowsM - 1) / kRowsM : 0;
+    }
+    tiles += wave_sum_i(c);
+  }
+  const int64_t row = static_cast<int64_t>(max(offsets[groups], 0)) + static_cast<int64_t>(chunk - tiles) * kRowsM +
+                      threadIdx.x / kRowsN;
+  const int col = ct * kRowsN + threadIdx.x % kRowsN;
+  if (row >= rows || col >= n) return;
+  if (out_dtype == QW_F32) static_cast<float*>(out)[row * n + col] = 0.0f;
+  else static_cast<uint16_t*>(out)[row * n + col] = 0;
+}
+
 template <int XDT, bool GATEUP>
 __global__ __launch_bounds__(kRowsThreads) void mx_rows_kernel(
     const void* __restrict__ x, int64_t x_stride, bool x_aligned, const uint8_t* __restrict__ x_scales,
     const int32_t* __restrict__ row_index, const int32_t* __restrict__ offsets, int groups, int rows, MxMatrix wa,
-    MxMatrix wb, int n, int k, int col_tiles, void* __restrict__ out, int out_dtype, uint8_t* __restrict__ h_codes,
+    MxMatrix wb, int n, int k, int col_tiles, void* __restrict__ out, int out_dtype, bool zero_rest, uint8_t* __restrict__ h_codes,
     uint8_t* __restrict__ h_scales) {
   constexpr int TILES = GATEUP ? 4 : 2;  // 16 weight rows each: two of gate, two of up
   __shared__ f32x4 part[kRowsWaves][TILES][kWave];
@@ -33,7 +55,10 @@ __global__ __launch_bounds__(kRowsThreads) void mx_rows_kernel(
   int r0 = chunk * kRowsM, end = rows;
   if (offsets) {
     e = find_tile(offsets, groups, rows, kRowsM, chunk, &local);
-    if (e < 0) return;
+    if (e < 0) {
+      if (!GATEUP && zero_rest) zero_rows(offsets, groups, rows, chunk, ct, n, out, out_dtype);
+      return;
+    }
     r0 = max(offsets[e], 0) + local * kRowsM;
     end = min(offsets[e + 1], rows);
   }
@@ -132,7 +157,7 @@ int launch_t(const MxProduct& p, hipStream_t stream) {
   const bool gateup = p.h_codes != nullptr;
   // hidden rows are written to their padded width
   const int64_t col_tiles = ceil_div(gateup ? mx_padded(p.n) : p.n, kRowsN);
-  const int64_t chunks = p.offsets ? ceil_div(p.rows, kRowsM) + p.groups : ceil_div(p.rows, kRowsM);
+  const int64_t chunks = p.offsets ? ceil_div(p.rows, kRowsM) + p.groups + (p.zero_rest ? 1 : 0) : ceil_div(p.rows, kRowsM);
   const int64_t grid = col_tiles * chunks;
   if (grid > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many rows and columns for one microscaled product");
   const int size = XDT == QW_F32 ? 4 : 2;
@@ -142,7 +167,7 @@ int launch_t(const MxProduct& p, hipStream_t stream) {
     kernel<<<static_cast<unsigned>(grid), kRowsThreads, 0, stream>>>(
         x, p.x_stride, aligned, p.x_scales, p.row_index, p.offsets, static_cast<int>(p.groups),
         static_cast<int>(p.rows), p.a, p.b, static_cast<int>(p.n), static_cast<int>(p.k), static_cast<int>(col_tiles),
-        p.out, p.out_dtype, p.h_codes, p.h_scales);
+        p.out, p.out_dtype, p.zero_rest, p.h_codes, p.h_scales);
   };
   if (gateup) go(mx_rows_kernel<XDT, true>);
   else go(mx_rows_kernel<XDT, false>);

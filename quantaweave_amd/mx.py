@@ -190,13 +190,13 @@ def mx_grouped_swiglu(x: Tensor, gate: tuple, up: tuple, down: tuple, offsets: T
         raise ValueError(f"{what}: max_rows must be >= 0")
     flat, stride = _rows(x, what)
     rows = flat.size(0)
-    out = torch.zeros(rows, d, dtype=x.dtype, device=x.device)
+    out = torch.empty(rows, d, dtype=x.dtype, device=x.device)
     if rows:
         offsets = offsets.contiguous()
-        nbytes = _lib.load().qw_mx_experts_workspace_bytes(rows, rows, experts, d, ffn)
+        nbytes = _lib.load().qw_mx_experts_workspace_bytes(rows, experts, d, ffn)
         ws = _hip.workspace(nbytes, x.device)
         _hip.call_on(x.device, "qw_mx_experts", _hip.ptr(flat), act, rows, stride, None, _hip.ptr(offsets), experts, d,
                      ffn, rows, min(max_rows or 0, rows), _hip.ptr(gate[0]), _hip.ptr(gate[1]), _hip.ptr(up[0]),
-                     _hip.ptr(up[1]), _hip.ptr(down[0]), _hip.ptr(down[1]), _hip.ptr(out), _hip.ptr(ws), nbytes,
+                     _hip.ptr(up[1]), _hip.ptr(down[0]), _hip.ptr(down[1]), 1, _hip.ptr(out), _hip.ptr(ws), nbytes,
                      _hip.stream(x.device))
     return out

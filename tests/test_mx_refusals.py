@@ -57,12 +57,12 @@ def test_entry_points_check_their_arguments_before_any_launch():
     refused(lib.qw_mx_dequantize(one, 66, 4, 64, one, 0, None), b"on 4")
     refused(lib.qw_mx_matmul(one, 1, 64, 4, None, one, 8, 64, one, None, 0, None), b"weight")
     refused(lib.qw_mx_matmul(one, 1, 64, -1, one, one, 8, 64, one, None, 0, None), b"rows")
-    refused(lib.qw_mx_experts(one, 1, 3, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, one, one, 1 << 30,
+    refused(lib.qw_mx_experts(one, 1, 3, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, 0, one, one, 1 << 30,
                               None), b"rows")
-    refused(lib.qw_mx_experts(one, 1, 4, 64, None, one, 0, 64, 64, 4, 0, one, one, one, one, one, one, one, one, 1 << 30,
+    refused(lib.qw_mx_experts(one, 1, 4, 64, None, one, 0, 64, 64, 4, 0, one, one, one, one, one, one, 0, one, one, 1 << 30,
                               None), b"experts")
-    need = lib.qw_mx_experts_workspace_bytes(4, 4, 2, 64, 64)
-    assert lib.qw_mx_experts(one, 1, 4, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, one, one,
+    need = lib.qw_mx_experts_workspace_bytes(4, 2, 64, 64)
+    assert lib.qw_mx_experts(one, 1, 4, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, 0, one, one,
                              need - 1, None) == _lib.QW_ERR_WORKSPACE
     need = lib.qw_mx_matmul_backward_workspace_bytes(4, 8, 64, 1)
     assert lib.qw_mx_matmul_backward(one, 1, 4, one, one, 8, 64, one, one, need - 1, None) == _lib.QW_ERR_WORKSPACE
