@@ -80,7 +80,7 @@ int qw_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_
 }
 
 size_t qw_mx_matmul_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features) {
-  if (rows < 1 || out_features < 1 || in_features < 1 || mx_few_rows(rows, 1)) return 0;
+  if (rows < 1 || out_features < 1 || in_features < 1) return 0;
   Carver c(nullptr);
   c.take<char>(static_cast<size_t>(rows) * mx_code_bytes(in_features));
   c.take<char>(static_cast<size_t>(rows) * mx_scale_bytes(in_features));
@@ -101,22 +101,27 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
   st = check_matrix(codes, scales, "weight");
   if (st) return st;
   const size_t need = qw_mx_matmul_workspace_bytes(rows, out_features, in_features);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+  const bool few = mx_few_rows(rows, 1), direct = few && mx_rows_takes(x, act_dtype, x_row_stride, in_features);
+  if (!direct && (workspace == nullptr || workspace_bytes < need))
     return set_error(QW_ERR_WORKSPACE, "mx_matmul needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
   MxProduct p;
   p.rows = rows, p.n = out_features, p.k = in_features;
   p.a = matrix(codes, scales);
   p.out = out, p.out_dtype = act_dtype;
-  if (need == 0) {
+  if (direct) {
     p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride;
     return launch_mx_rows(p, as_stream(stream));
   }
   Carver c(workspace);
   uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(rows) * mx_code_bytes(in_features));
   uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(rows) * mx_scale_bytes(in_features));
+  p.x_codes = xq, p.x_scales = xs;
+  if (few) {
+    st = mx_quantize(x, act_dtype, rows, in_features, x_row_stride, xq, xs, as_stream(stream));
+    return st ? st : launch_mx_rows(p, as_stream(stream));
+  }
   st = mx_prepare(x, act_dtype, rows, in_features, x_row_stride, xq, xs, MxPrepare(), as_stream(stream));
   if (st) return st;
-  p.x_codes = xq, p.x_scales = xs;
   p.chunk_rows = mx_dense_chunk(rows, out_features);
   return launch_mx_gemm(p, as_stream(stream));
 }
@@ -164,9 +169,9 @@ size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t 
   Carver c(nullptr);
   c.take<char>(static_cast<size_t>(max_rows) * mx_code_bytes(d_ff));
   c.take<char>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_ff));
+  c.take<char>(static_cast<size_t>(max_rows) * mx_code_bytes(d_model));
+  c.take<char>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_model));
   if (!mx_few_rows(max_rows, experts)) {
-    c.take<char>(static_cast<size_t>(max_rows) * mx_code_bytes(d_model));
-    c.take<char>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_model));
     c.take<int4>(static_cast<size_t>(mx_max_chunks(max_rows, experts, 64)) + 1);  // the smallest chunks
   }
   return c.used + 256;
@@ -208,14 +213,21 @@ int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_st
   d.n = d_model, d.k = d_ff;
   d.a = matrix(down_codes, down_scales);
   d.out = y, d.out_dtype = act_dtype;
+  uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_code_bytes(d_model));
+  uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_model));
   if (mx_few_rows(max_rows, experts)) {
-    p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride, p.row_index = row_index;
+    if (mx_rows_takes(x, act_dtype, x_row_stride, d_model)) {
+      p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride, p.row_index = row_index;
+    } else {
+      st = mx_gather(x, act_dtype, max_rows, d_model, x_row_stride, row_index, kept_offsets + experts, xq, xs,
+                     as_stream(stream));
+      if (st) return st;
+      p.x_codes = xq, p.x_scales = xs;
+    }
     st = launch_mx_rows(p, as_stream(stream));
     d.zero_rest = zero_rest != 0;
     return st ? st : launch_mx_rows(d, as_stream(stream));
   }
-  uint8_t* xq = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_code_bytes(d_model));
-  uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_model));
   const int64_t cap = max_rows_per_expert > 0 && max_rows_per_expert < max_rows ? max_rows_per_expert : max_rows;
   MxPrepare prep;
   prep.row_index = row_index, prep.offsets = kept_offsets, prep.groups = experts;

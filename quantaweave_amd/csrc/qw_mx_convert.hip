@@ -31,44 +31,84 @@ __device__ void chunk_table(const int32_t* __restrict__ offsets, int groups, int
 }
 
 // Four lanes make a block: each loads eight consecutive numbers (16 bytes of a
-// 16-bit type), the largest magnitude goes round the four with two DPP moves,
-// each stores four bytes of codes and the first the scale byte.  Padding columns
-// are written as zeros.  Bound by HBM (8192 x 2048 bf16, 42 MB: 9.4 us, 4.5 TB/s;
-// a copy reaches 5.1).  PREPARE: rows for the tile kernel: gathered, the scales step
-// by step, the last workgroup making the chunk table, rows of no group skipped
-// and their results zeroed.
-template <int DT, bool PREPARE>
-__global__ __launch_bounds__(kConvertThreads) void mx_quantize_kernel(const void* __restrict__ x, int64_t stride,
-                                                                      int rows, int cols, uint32_t pieces,
-                                                                      int64_t total, bool aligned, MxPrepare prep,
-                                                                      int most, uint32_t* __restrict__ codes,
-                                                                      uint8_t* __restrict__ scales) {
-  if (PREPARE && prep.table != nullptr && blockIdx.x == gridDim.x - 1) {
-    chunk_table(prep.offsets, static_cast<int>(prep.groups), rows, prep.chunk_rows, most, prep.table);
-    return;
-  }
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvertThreads + threadIdx.x;
-  if (i >= total) return;  // whole blocks: total is a multiple of 16 and the four lanes of a block go together
-  const int64_t row = total <= INT32_MAX ? static_cast<uint32_t>(i) / pieces : i / pieces;
-  const int piece = static_cast<int>(i - row * pieces), col = piece * 8;
-  int64_t src = row;
-  if constexpr (PREPARE) {
-    if (prep.offsets != nullptr && row >= prep.offsets[prep.groups]) {
-      if (prep.zero_out != nullptr)
-        for (int k = 0; k < 8 && col + k < cols; ++k) store_act<DT>(prep.zero_out, row * cols + col + k, 0.0f);
-      return;
-    }
-    if (prep.row_index != nullptr) src = prep.row_index[row];
-  }
-  const MxPiece<DT> v = mx_load_piece<DT>(x, src * stride + col, cols - col, aligned);
+// 16-bit type), the largest magnitude goes round the four with two DPP moves.
+template <int DT>
+__device__ __forceinline__ uint32_t block_scale(const MxPiece<DT>& v) {
   uint32_t top = mx_piece_top<DT>(v);
   top = mx_top_max<DT>(top, dpp_u32<kDppXor1>(top));
   top = mx_top_max<DT>(top, dpp_u32<kDppXor2>(top));
-  const uint32_t s = mx_scale_of(mx_top_bits<DT>(top));
+  return mx_scale_of(mx_top_bits<DT>(top));
+}
+
+// Each lane stores four bytes of codes, a block's first lane its scale byte.
+// Padding columns are written as zeros.  Bound by HBM (8192 x 2048 bf16, 42 MB:
+// 9.4 us, 4.5 TB/s; a copy reaches 5.1).
+template <int DT>
+__global__ __launch_bounds__(kConvertThreads) void mx_quantize_kernel(const void* __restrict__ x, int64_t stride,
+                                                                      int cols, uint32_t pieces, int64_t total,
+                                                                      bool aligned, const int32_t* __restrict__ index,
+                                                                      const int32_t* __restrict__ end,
+                                                                      uint32_t* __restrict__ codes,
+                                                                      uint8_t* __restrict__ scales) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvertThreads + threadIdx.x;
+  if (i >= total) return;  // whole blocks: total is a multiple of 16 and the four lanes of a block go together
+  const int64_t row = total <= INT32_MAX ? static_cast<uint32_t>(i) / pieces : i / pieces;
+  const int col = static_cast<int>(i - row * pieces) * 8;
+  if (end != nullptr && row >= *end) return;  // rows that index says nothing of
+  const int64_t src = index != nullptr ? index[row] : row;
+  const MxPiece<DT> v = mx_load_piece<DT>(x, src * stride + col, cols - col, aligned);
+  const uint32_t s = block_scale<DT>(v);
   codes[i] = mx_piece_codes<DT>(v, s);
-  if (threadIdx.x % 4 == 0) {
-    if constexpr (PREPARE) scales[(static_cast<int64_t>(piece / 16) * rows + row) * 4 + piece / 4 % 4] = static_cast<uint8_t>(s);
-    else scales[i / 4] = static_cast<uint8_t>(s);
+  if (threadIdx.x % 4 == 0) scales[i / 4] = static_cast<uint8_t>(s);
+}
+
+// Rows for the tile kernel: gathered, the scales step by step.  A workgroup holds
+// sixteen rows by sixteen lanes, a step of 128 columns, and goes through up to
+// kPrepareSteps of them: the scales of a step are one dword per row, sixteen rows
+// side by side.  The last workgroup makes the chunk table; rows of no group are
+// skipped and their results zeroed.
+constexpr int kPrepareRows = 16, kPrepareSteps = 4;
+
+template <int DT>
+__global__ __launch_bounds__(kConvertThreads) void mx_prepare_kernel(const void* __restrict__ x, int64_t stride,
+                                                                     int rows, int cols, int steps, int step_groups,
+                                                                     bool aligned, MxPrepare prep, int most,
+                                                                     uint32_t* __restrict__ codes,
+                                                                     uint32_t* __restrict__ scales) {
+  if (prep.table != nullptr && blockIdx.x == gridDim.x - 1) {
+    chunk_table(prep.offsets, static_cast<int>(prep.groups), rows, prep.chunk_rows, most, prep.table);
+    return;
+  }
+  const int row = static_cast<int>(blockIdx.x / step_groups) * kPrepareRows + threadIdx.x / 16;
+  const int s0 = static_cast<int>(blockIdx.x % step_groups) * kPrepareSteps;
+  if (row >= rows) return;  // sixteen lanes together
+  const int piece = threadIdx.x % 16;
+  if (prep.offsets != nullptr && row >= prep.offsets[prep.groups]) {
+    if (prep.zero_out != nullptr)
+      for (int j = 0; j < kPrepareSteps; ++j)
+        for (int k = 0; k < 8; ++k) {
+          const int col = (s0 + j) * kMxStep + piece * 8 + k;
+          if (col < cols) store_act<DT>(prep.zero_out, static_cast<int64_t>(row) * cols + col, 0.0f);
+        }
+    return;
+  }
+  const int64_t src = prep.row_index != nullptr ? prep.row_index[row] : row;
+  MxPiece<DT> v[kPrepareSteps];
+#pragma unroll
+  for (int j = 0; j < kPrepareSteps; ++j) {
+    const int col = (s0 + j) * kMxStep + piece * 8;
+    v[j] = mx_load_piece<DT>(x, src * stride + col, cols - col, aligned);
+  }
+#pragma unroll
+  for (int j = 0; j < kPrepareSteps; ++j) {
+    if (s0 + j >= steps) break;
+    uint32_t s = block_scale<DT>(v[j]);
+    codes[static_cast<int64_t>(row) * steps * 16 + (s0 + j) * 16 + piece] = mx_piece_codes<DT>(v[j], s);
+    // the four blocks' bytes meet in the step's first lane
+    s <<= 8 * (piece / 4);
+    s |= dpp_u32<kDppHalfMirror>(s);
+    s |= dpp_u32<kDppMirror>(s);
+    if (piece == 0) scales[static_cast<int64_t>(s0 + j) * rows + row] = s;
   }
 }
 
@@ -106,37 +146,51 @@ __global__ __launch_bounds__(kConvertThreads) void mx_dequantize_kernel(const ui
 
 }  // namespace
 
-template <bool PREPARE>
-static int launch_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes,
-                           void* scales, const MxPrepare& prep, hipStream_t stream) {
+int mx_gather(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, const int32_t* index,
+              const int32_t* end, void* codes, void* scales, hipStream_t stream) {
   const int64_t pieces = mx_padded(cols) / 8, total = rows * pieces;
   if (total == 0) return QW_OK;
-  const int64_t blocks = ceil_div(total, kConvertThreads) + (PREPARE && prep.table ? 1 : 0);
-  if (blocks > INT32_MAX || rows > INT32_MAX)
-    return set_error(QW_ERR_UNSUPPORTED, "too many rows to quantise in one call");
+  const int64_t blocks = ceil_div(total, kConvertThreads);
+  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many rows to quantise in one call");
   const int size = dtype == QW_F32 ? 4 : 2;
   const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * size % 16 == 0;
-  const int most = PREPARE && prep.table ? static_cast<int>(mx_max_chunks(rows, prep.groups, prep.chunk_rows)) : 0;
   auto go = [&](auto kernel) {
     kernel<<<static_cast<unsigned>(blocks), kConvertThreads, 0, stream>>>(
-        x, stride, static_cast<int>(rows), static_cast<int>(cols), static_cast<uint32_t>(pieces), total, aligned, prep,
-        most, static_cast<uint32_t*>(codes), static_cast<uint8_t*>(scales));
+        x, stride, static_cast<int>(cols), static_cast<uint32_t>(pieces), total, aligned, index,
+        end, static_cast<uint32_t*>(codes), static_cast<uint8_t*>(scales));
   };
-  if (dtype == QW_F32) go(mx_quantize_kernel<QW_F32, PREPARE>);
-  else if (dtype == QW_F16) go(mx_quantize_kernel<QW_F16, PREPARE>);
-  else go(mx_quantize_kernel<QW_BF16, PREPARE>);
+  if (dtype == QW_F32) go(mx_quantize_kernel<QW_F32>);
+  else if (dtype == QW_F16) go(mx_quantize_kernel<QW_F16>);
+  else go(mx_quantize_kernel<QW_BF16>);
   QW_LAUNCH_CHECK("mx_quantize_kernel");
   return QW_OK;
 }
 
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
                 hipStream_t stream) {
-  return launch_quantize<false>(x, dtype, rows, cols, stride, codes, scales, MxPrepare(), stream);
+  return mx_gather(x, dtype, rows, cols, stride, nullptr, nullptr, codes, scales, stream);
 }
 
 int mx_prepare(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, uint8_t* codes, uint8_t* scales,
                const MxPrepare& prep, hipStream_t stream) {
-  return launch_quantize<true>(x, dtype, rows, cols, stride, codes, scales, prep, stream);
+  if (rows == 0) return QW_OK;
+  const int64_t steps = mx_padded(cols) / kMxStep, step_groups = ceil_div(steps, kPrepareSteps);
+  const int64_t blocks = ceil_div(rows, kPrepareRows) * step_groups + (prep.table ? 1 : 0);
+  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many rows to quantise in one call");
+  const int size = dtype == QW_F32 ? 4 : 2;
+  const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * size % 16 == 0;
+  const int most = prep.table ? static_cast<int>(mx_max_chunks(rows, prep.groups, prep.chunk_rows)) : 0;
+  auto go = [&](auto kernel) {
+    kernel<<<static_cast<unsigned>(blocks), kConvertThreads, 0, stream>>>(
+        x, stride, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(steps),
+        static_cast<int>(step_groups), aligned, prep, most, reinterpret_cast<uint32_t*>(codes),
+        reinterpret_cast<uint32_t*>(scales));
+  };
+  if (dtype == QW_F32) go(mx_prepare_kernel<QW_F32>);
+  else if (dtype == QW_F16) go(mx_prepare_kernel<QW_F16>);
+  else go(mx_prepare_kernel<QW_BF16>);
+  QW_LAUNCH_CHECK("mx_prepare_kernel");
+  return QW_OK;
 }
 
 int mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,

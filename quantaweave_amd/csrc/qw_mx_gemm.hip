@@ -223,9 +223,9 @@ __global__ __launch_bounds__(MX_THREADS) void mx_gemm_kernel(
     u32x4 xq[UNITS + 2], w1[2], wn[2];
     uint32_t sq[UNITS + 2], wsn[2];  // the scale of a unit; both steps of a tile share it
     xq[0] = x[0], xq[1] = x[1], sq[0] = xs[0], sq[1] = xs[1];
-    request();
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
+      if (u == 1) request();
       const int i = u % NPA;
       auto multiply = [&](int t) {
         if (u < NPA) acc[i][t] = mx_mfma32<0>(w[t], xq[u], acc[i][t], ws[t], sq[u]);

@@ -42,6 +42,8 @@ struct MxProduct {
 };
 
 // Few rows per group: weights streamed, K split over the waves of a workgroup.
+// Rows as numbers have to be ones that mx_rows_takes.
+bool mx_rows_takes(const void* x, int dtype, int64_t stride, int64_t k);
 int launch_mx_rows(const MxProduct& p, hipStream_t stream);
 // Many rows (stored ones): tiles of the matrix instruction through LDS.
 int launch_mx_gemm(const MxProduct& p, hipStream_t stream);
@@ -68,6 +70,9 @@ int mx_prepare(const void* x, int dtype, int64_t rows, int64_t cols, int64_t str
 
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
                 hipStream_t stream);
+// The same of the rows x[index[r]] (NULL: x[r]) for r < *end (device; NULL: all).
+int mx_gather(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, const int32_t* index,
+              const int32_t* end, void* codes, void* scales, hipStream_t stream);
 int mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
                   hipStream_t stream);
 

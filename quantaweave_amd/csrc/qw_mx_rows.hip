@@ -1,154 +1,195 @@
 // Microscaled products of few rows (decoding): each weight is read once per
 // sixteen rows of its group, straight from memory into the matrix instruction.
 //
-// One workgroup of eight waves owns sixteen rows of a group and 32 columns of
-// the result (two matrices: 32 gate and the matching 32 up columns, one block of
-// the hidden row).  A wave takes every eighth step of 128 columns: its lanes hold
-// 16 weight rows by four blocks, one 16-byte load and one scale byte per lane and
-// 16 columns of the result; rows given as numbers become codes in the registers
-// of the lane that multiplies them, whose 32 numbers are one block.  The eight
-// partial sums meet in LDS and are added in wave order (the same sum whatever
-// the rows beside it).  Bound by HBM where all experts are touched, by latency
-// for a single matrix.
+// One workgroup owns sixteen rows of a group and 32 columns of the result (two
+// matrices: 32 gate and the matching 32 up columns, one block of the hidden row).
+// The K axis is split over its waves in pairs of steps, 256 columns, so that a
+// wave's two loads of a weight row are one 128-byte line and the pair's scales
+// eight bytes: its lanes hold 16 weight rows by four blocks, one 16-byte load per
+// lane, step and 16 columns of the result.  A pair's loads go out together, with
+// one matrix before the rows are looked at.
+// Rows given as numbers become codes in the registers of the lane that multiplies
+// them, whose 32 numbers are one block.  The partial sums meet in LDS and are added
+// in wave order (the same sum whatever the rows beside it).
+//
+// Bound by the weight stream where many experts are touched (@EXPERTS@), by latency
+// for a single matrix (1 row, 2048 x 7168: @ONE@).
 #include "qw_mx_product.h"
 
 namespace qw {
 
 namespace {
 
-constexpr int kRowsWaves = 8, kRowsThreads = kRowsWaves * kWave;
 constexpr int kRowsM = 16, kRowsN = 32;
 constexpr int kStored = -1;  // XDT of rows that are stored microscaled
+constexpr int kRowsLayers = 2;  // workgroups that share a group's row chunks
 
-// The workgroups past the groups' last tile: zeros in the rows behind the last
-// group, sixteen rows by 32 columns each.
-__device__ void zero_rows(const int32_t* __restrict__ offsets, int groups, int rows, int chunk, int ct, int n,
-                          void* __restrict__ out, int out_dtype) {
-  const int lane = threadIdx.x % kWave;
-  int tiles = 0;
-  for (int e0 = 0; e0 < groups; e0 += kWave) {
-    int c = 0;
-    if (e0 + lane < groups) {
-      const int lo = min(max(offsets[e0 + lane], 0), rows), hi = min(offsets[e0 + lane + 1], rows);
-      c = hi > lo ? (hi - lo + kRowsM - 1) / kRowsM : 0;
-    }
-    tiles += wave_sum_i(c);
+// Eight numbers from element i (on 16 bytes), or zeros.
+template <int DT>
+__device__ __forceinline__ MxPiece<DT> whole_piece(const void* __restrict__ p, int64_t i, bool there) {
+  MxPiece<DT> r;
+  uint4 a = make_uint4(0, 0, 0, 0), b = a;
+  if (there) {
+    const uint4* const at = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (DT == QW_F32 ? 4 : 2));
+    a = at[0];
+    if constexpr (DT == QW_F32) b = at[1];
   }
-  const int64_t row = static_cast<int64_t>(max(offsets[groups], 0)) + static_cast<int64_t>(chunk - tiles) * kRowsM +
-                      threadIdx.x / kRowsN;
-  const int col = ct * kRowsN + threadIdx.x % kRowsN;
-  if (row >= rows || col >= n) return;
-  if (out_dtype == QW_F32) static_cast<float*>(out)[row * n + col] = 0.0f;
-  else static_cast<uint16_t*>(out)[row * n + col] = 0;
+  r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+  if constexpr (DT == QW_F32) r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
+  return r;
 }
 
-template <int XDT, bool GATEUP>
-__global__ __launch_bounds__(kRowsThreads) void mx_rows_kernel(
-    const void* __restrict__ x, int64_t x_stride, bool x_aligned, const uint8_t* __restrict__ x_scales,
+template <int XDT, bool GATEUP, int WAVES>
+__global__ __launch_bounds__(WAVES* kWave, 4) void mx_rows_kernel(
+    const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ x_scales,
     const int32_t* __restrict__ row_index, const int32_t* __restrict__ offsets, int groups, int rows, MxMatrix wa,
-    MxMatrix wb, int n, int k, int col_tiles, void* __restrict__ out, int out_dtype, bool zero_rest, uint8_t* __restrict__ h_codes,
-    uint8_t* __restrict__ h_scales) {
+    MxMatrix wb, int n, int k, int col_tiles, int layers, void* __restrict__ out, int out_dtype, bool zero_rest,
+    uint8_t* __restrict__ h_codes, uint8_t* __restrict__ h_scales) {
   constexpr int TILES = GATEUP ? 4 : 2;  // 16 weight rows each: two of gate, two of up
-  __shared__ f32x4 part[kRowsWaves][TILES][kWave];
-  const int ct = blockIdx.x % col_tiles, chunk = blockIdx.x / col_tiles;
-  int e = 0, local = chunk;
-  int r0 = chunk * kRowsM, end = rows;
+  constexpr int THREADS = WAVES * kWave;
+  // Two matrices' fragments and the numbers of a row together do not fit the
+  // registers of two workgroups per unit: there the rows come first.
+  constexpr bool kRowsFirst = GATEUP && XDT != kStored;
+  __shared__ f32x4 part[WAVES][TILES][kWave];
+  const int ct = blockIdx.x % col_tiles, place = blockIdx.x / col_tiles;
+  const int e = offsets ? place % groups : 0, layer = offsets ? place / groups : place;
+  int lo = 0, end = rows;
   if (offsets) {
-    e = find_tile(offsets, groups, rows, kRowsM, chunk, &local);
-    if (e < 0) {
-      if (!GATEUP && zero_rest) zero_rows(offsets, groups, rows, chunk, ct, n, out, out_dtype);
-      return;
-    }
-    r0 = max(offsets[e], 0) + local * kRowsM;
+    lo = max(offsets[e], 0);
     end = min(offsets[e + 1], rows);
   }
-  const int count = min(end - r0, kRowsM);
-  if (count <= 0) return;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int l16 = lane % 16, lq = lane / 16;
   const int n0 = ct * kRowsN;
   const int64_t pitch = (k + kMxStep - 1) / kMxStep * static_cast<int64_t>(kMxStep);
   const int64_t cb = pitch / 2, sb = pitch / kMxBlock;
-  const int steps = static_cast<int>(pitch / kMxStep);
+  const int steps = static_cast<int>(pitch / kMxStep), pairs = (steps + 1) / 2;
 
-  // rows past the count repeat the last one; their results are not stored
-  const int rr = r0 + min(l16, count - 1);
-  const int64_t row = row_index ? row_index[rr] : rr;
-  const uint8_t* w_codes[TILES];
-  const uint8_t* w_scales[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const MxMatrix& m = t < 2 ? wa : wb;
-    const int64_t wr = static_cast<int64_t>(e) * n + min(n0 + (t % 2) * 16 + l16, n - 1);
-    w_codes[t] = m.codes + wr * cb + lq * 16;
-    w_scales[t] = m.scales + wr * sb + lq;
+  if (!GATEUP && zero_rest && offsets) {  // the rows behind the last group, shared by all workgroups
+    for (int64_t r0 = static_cast<int64_t>(max(offsets[groups], 0)) + place * kRowsM; r0 < rows;
+         r0 += static_cast<int64_t>(groups) * layers * kRowsM)
+      for (int i = tid; i < kRowsM * kRowsN; i += THREADS) {
+        const int64_t row = r0 + i / kRowsN;
+        const int col = n0 + i % kRowsN;
+        if (row >= rows || col >= n) continue;
+        if (out_dtype == QW_F32) static_cast<float*>(out)[row * n + col] = 0.0f;
+        else static_cast<uint16_t*>(out)[row * n + col] = 0;
+      }
   }
-  f32x4 acc[TILES];
+  // a matrix's rows of this workgroup: uniform bases, a lane's two row offsets.  Rows
+  // past the matrix repeat its last one; a tile of padding columns alone (hidden rows
+  // are written to their padded width) lies on it wholly.  Their results are not used.
+  const int first_row = min(n0, n - 1);
+  const int64_t w0 = static_cast<int64_t>(e) * n + first_row;
+  const uint8_t* const codes[2] = {wa.codes + w0 * cb, GATEUP ? wb.codes + w0 * cb : nullptr};
+  const uint8_t* const scales[2] = {wa.scales + w0 * sb, GATEUP ? wb.scales + w0 * sb : nullptr};
+  uint32_t w_off[2], s_off[2];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = wave; s < steps; s += kRowsWaves) {
-    u32x4 w[TILES];
-    uint32_t ws[TILES];
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      w[t] = *reinterpret_cast<const u32x4*>(w_codes[t] + static_cast<int64_t>(s) * 64);
-      ws[t] = w_scales[t][s * 4];
-    }
-    u32x4 xc;
-    uint32_t xs;
-    if constexpr (XDT == kStored) {
-      xc = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(x) + row * cb + s * 64 + lq * 16);
-      xs = x_scales[row * sb + s * 4 + lq];
-    } else {
-      const int col = s * kMxStep + lq * kMxBlock;
-      MxPiece<XDT> v[4];
-      uint32_t top = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        v[q] = mx_load_piece<XDT>(x, row * x_stride + col + 8 * q, k - col - 8 * q, x_aligned);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) top = mx_top_max<XDT>(top, mx_piece_top<XDT>(v[q]));
-      xs = mx_scale_of(mx_top_bits<XDT>(top));
-#pragma unroll
-      for (int q = 0; q < 4; ++q) xc[q] = mx_piece_codes<XDT>(v[q], xs);
-    }
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma(w[t], xc, acc[t], ws[t], xs);
+  for (int t = 0; t < 2; ++t) {
+    const uint32_t r = min(t * 16 + l16, n - 1 - first_row);
+    w_off[t] = r * static_cast<uint32_t>(cb) + lq * 16;
+    s_off[t] = r * static_cast<uint32_t>(sb);
   }
+  for (int64_t r0 = lo + static_cast<int64_t>(layer) * kRowsM; r0 < end; r0 += static_cast<int64_t>(layers) * kRowsM) {
+    const int count = min(static_cast<int>(end - r0), kRowsM);
+    f32x4 acc[TILES];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) part[wave][t][lane] = acc[t];
-  __syncthreads();
-  // thread -> (row m, column c): a lane's four sums are columns 4 lq .. 4 lq + 3 of row l16
-  const int m = tid / kRowsN, c = tid % kRowsN;
-  auto total = [&](int t) {
-    const int at = m + 16 * (c % 16 / 4);
-    float v = part[0][t][at][c % 4];
+    for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 w[TILES][2];
+    uint32_t ws[TILES][2];
+    // a pair of steps; where the last holds one, the second rereads it and is not multiplied
+    auto load = [&](int p) {
+      const int second = 2 * p + 1 < steps ? 1 : 0;
 #pragma unroll
-    for (int w = 1; w < kRowsWaves; ++w) v += part[w][t][at][c % 4];
-    return v;
-  };
-  const int64_t orow = r0 + m;
-  if constexpr (!GATEUP) {
-    const float v = total(c / 16);
-    if (m < count && n0 + c < n) {
-      if (out_dtype == QW_F32) store_act<QW_F32>(out, orow * n + n0 + c, v);
-      else if (out_dtype == QW_F16) store_act<QW_F16>(out, orow * n + n0 + c, v);
-      else store_act<QW_BF16>(out, orow * n + n0 + c, v);
+      for (int t = 0; t < TILES; ++t) {
+        const uint8_t* const c = codes[t / 2] + static_cast<int64_t>(p) * 128;
+        const uint8_t* const s = scales[t / 2] + static_cast<int64_t>(p) * 8;
+        w[t][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(c + w_off[t % 2]));
+        w[t][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(c + second * 64 + w_off[t % 2]));
+        ws[t][0] = *reinterpret_cast<const uint32_t*>(s + s_off[t % 2]);
+        ws[t][1] = *reinterpret_cast<const uint32_t*>(s + second * 4 + s_off[t % 2]);
+      }
+    };
+    int first = wave;
+    asm volatile("" : "+s"(first));  // the next chunk loads its weights again: kept, they would cost the registers twice
+    if (!kRowsFirst && first < pairs) load(first);
+    // rows past the count repeat the last one; their results are not stored
+    const int64_t rr = r0 + min(l16, count - 1);
+    const int64_t row = row_index ? row_index[rr] : rr;
+#pragma unroll 1
+    for (int p = first; p < pairs; p += WAVES) {
+      u32x4 xc[2];
+      uint32_t xs[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = min(2 * p + j, steps - 1);
+        if constexpr (XDT == kStored) {
+          xc[j] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(x) + row * cb + s * 64 + lq * 16);
+          xs[j] = x_scales[row * sb + s * 4 + lq];
+        } else {  // a block of this row; its pieces exist whole or not at all
+          const int col = s * kMxStep + lq * kMxBlock;
+          MxPiece<XDT> v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = whole_piece<XDT>(x, row * x_stride + col + 8 * q, col + 8 * q < k);
+          uint32_t top = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) top = mx_top_max<XDT>(top, mx_piece_top<XDT>(v[q]));
+          xs[j] = mx_scale_of(mx_top_bits<XDT>(top));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) xc[j][q] = mx_piece_codes<XDT>(v[q], xs[j]);
+        }
+      }
+      if (kRowsFirst) {
+        asm volatile("" ::: "memory");  // the rows' registers are free before the weights' are taken
+        load(p);
+      }
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma(w[t][0], xc[0], acc[t], ws[t][0] >> (8 * lq), xs[0]);
+      if (2 * p + 1 < steps)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma(w[t][1], xc[1], acc[t], ws[t][1] >> (8 * lq), xs[1]);
+      if (!kRowsFirst && p + WAVES < pairs) load(p + WAVES);
     }
-  } else {
-    const bool live = n0 + c < n;  // padding columns of the hidden row are zero codes
-    const float h = live ? mx_swiglu(total(c / 16), total(2 + c / 16)) : 0.0f;
-    uint32_t top = __float_as_uint(h) & 0x7fffffffu;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, kWave)));
-    const uint32_t s = mx_scale_of(top);
-    const float other = __shfl_xor(h, 1, kWave);
-    const uint32_t code = s == kMxNan ? 0u : mx_pack_f32<0>(0u, h, other, mx_divisor(s));
-    const int64_t np = (n + kMxStep - 1) / kMxStep * static_cast<int64_t>(kMxStep);
-    if (m < count) {
-      if (c % 2 == 0) h_codes[orow * (np / 2) + (n0 + c) / 2] = static_cast<uint8_t>(code);
-      if (c == 0) h_scales[orow * (np / kMxBlock) + n0 / kMxBlock] = static_cast<uint8_t>(s);
+    for (int t = 0; t < TILES; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    // thread -> (row m, column c): a lane's four sums are columns 4 lq .. 4 lq + 3 of row l16
+#pragma unroll
+    for (int i = tid; i < kRowsM * kRowsN; i += THREADS) {
+      const int m = i / kRowsN, c = i % kRowsN;
+      auto total = [&](int t) {
+        const int at = m + 16 * (c % 16 / 4);
+        float v = part[0][t][at][c % 4];
+#pragma unroll
+        for (int u = 1; u < WAVES; ++u) v += part[u][t][at][c % 4];
+        return v;
+      };
+      const int64_t orow = r0 + m;
+      if constexpr (!GATEUP) {
+        const float v = total(c / 16);
+        if (m < count && n0 + c < n) {
+          if (out_dtype == QW_F32) store_act<QW_F32>(out, orow * n + n0 + c, v);
+          else if (out_dtype == QW_F16) store_act<QW_F16>(out, orow * n + n0 + c, v);
+          else store_act<QW_BF16>(out, orow * n + n0 + c, v);
+        }
+      } else {
+        const bool live = n0 + c < n;  // padding columns of the hidden row are zero codes
+        const float h = live ? mx_swiglu(total(c / 16), total(2 + c / 16)) : 0.0f;
+        uint32_t top = __float_as_uint(h) & 0x7fffffffu;
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1)
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, kWave)));
+        const uint32_t s = mx_scale_of(top);
+        const float other = __shfl_xor(h, 1, kWave);
+        const uint32_t code = s == kMxNan ? 0u : mx_pack_f32<0>(0u, h, other, mx_divisor(s));
+        const int64_t np = (n + kMxStep - 1) / kMxStep * static_cast<int64_t>(kMxStep);
+        if (m < count) {
+          if (c % 2 == 0) h_codes[orow * (np / 2) + (n0 + c) / 2] = static_cast<uint8_t>(code);
+          if (c == 0) h_scales[orow * (np / kMxBlock) + n0 / kMxBlock] = static_cast<uint8_t>(s);
+        }
+      }
     }
+    if (r0 + static_cast<int64_t>(layers) * kRowsM < end) __syncthreads();  // the sums are read before the next chunk's
   }
 }
 
@@ -157,25 +198,32 @@ int launch_t(const MxProduct& p, hipStream_t stream) {
   const bool gateup = p.h_codes != nullptr;
   // hidden rows are written to their padded width
   const int64_t col_tiles = ceil_div(gateup ? mx_padded(p.n) : p.n, kRowsN);
-  const int64_t chunks = p.offsets ? ceil_div(p.rows, kRowsM) + p.groups + (p.zero_rest ? 1 : 0) : ceil_div(p.rows, kRowsM);
-  const int64_t grid = col_tiles * chunks;
+  const int64_t chunks = ceil_div(p.rows, kRowsM);
+  const int64_t layers = p.offsets ? std::min<int64_t>(chunks, kRowsLayers) : chunks;
+  const int64_t grid = col_tiles * layers * p.groups;
   if (grid > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many rows and columns for one microscaled product");
-  const int size = XDT == QW_F32 ? 4 : 2;
-  const bool aligned = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_stride * size % 16 == 0;
   const void* x = XDT == kStored ? p.x_codes : p.x;
-  auto go = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(grid), kRowsThreads, 0, stream>>>(
-        x, p.x_stride, aligned, p.x_scales, p.row_index, p.offsets, static_cast<int>(p.groups),
+  auto go = [&](auto kernel, int waves) {
+    kernel<<<static_cast<unsigned>(grid), waves * kWave, 0, stream>>>(
+        x, p.x_stride, p.x_scales, p.row_index, p.offsets, static_cast<int>(p.groups),
         static_cast<int>(p.rows), p.a, p.b, static_cast<int>(p.n), static_cast<int>(p.k), static_cast<int>(col_tiles),
-        p.out, p.out_dtype, p.zero_rest, p.h_codes, p.h_scales);
+        static_cast<int>(layers), p.out, p.out_dtype, p.zero_rest, p.h_codes, p.h_scales);
   };
-  if (gateup) go(mx_rows_kernel<XDT, true>);
-  else go(mx_rows_kernel<XDT, false>);
+  // a wave per pair of steps up to eight: more waves than pairs would idle
+  const bool eight = mx_padded(p.k) > 4 * 2 * kMxStep;
+  if (gateup && eight) go(mx_rows_kernel<XDT, true, 8>, 8);
+  else if (gateup) go(mx_rows_kernel<XDT, true, 4>, 4);
+  else if (eight) go(mx_rows_kernel<XDT, false, 8>, 8);
+  else go(mx_rows_kernel<XDT, false, 4>, 4);
   QW_LAUNCH_CHECK("mx_rows_kernel");
   return QW_OK;
 }
 
 }  // namespace
+
+bool mx_rows_takes(const void* x, int dtype, int64_t stride, int64_t k) {
+  return reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * (dtype == QW_F32 ? 4 : 2) % 16 == 0 && k % 8 == 0;
+}
 
 int launch_mx_rows(const MxProduct& p, hipStream_t stream) {
   if (p.x_codes) return launch_t<kStored>(p, stream);
