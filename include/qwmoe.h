@@ -476,32 +476,21 @@ int qw_moe_route_backward(const float* probs, const int32_t* top_idx, const floa
  *   top_idx = the top_k highest choices among them, descending       [T, k]
  *   top_w  = scores[top_idx] / (their sum + 1e-20) * scale, or without the
  *            division when renormalize == 0                          [T, k]
- *   probs  = scores / sum(scores) (NULL: not wanted; all 0 without a sum)
  * The choice is that of 64-bit arithmetic on the logits; equal values go to the
  * lowest index, a NaN counts as -infinity.  A softmax row of -infinities has
  * scores 0.  1 <= experts <= 1024, groups divides experts, top_k <= 64 and at
  * most the experts of top_groups groups. */
 int qw_moe_route_scored_from_logits(const float* logits, int64_t tokens, int64_t experts, int64_t top_k, int score,
                                     const float* bias, int64_t groups, int64_t top_groups, int group_top,
-                                    int renormalize, float scale, float* scores, float* probs, int32_t* top_idx,
-                                    float* top_w, void* stream);
+                                    int renormalize, float scale, float* scores, int32_t* top_idx, float* top_w,
+                                    void* stream);
 
-/* The same behind the router's product: logits = x @ router_w^T / temperature,
- * as qw_moe_route forms and stores them (its workspace). */
-int qw_moe_route_scored(const void* x, int x_dtype, int64_t x_row_stride, const void* router_w, int w_dtype,
-                        int64_t tokens, int64_t d_model, int64_t experts, int64_t top_k, float temperature, int score,
-                        const float* bias, int64_t groups, int64_t top_groups, int group_top, int renormalize,
-                        float scale, float* logits, float* scores, float* probs, int32_t* top_idx, float* top_w,
-                        void* workspace, size_t workspace_bytes, void* stream);
-
-/* Its gradient with respect to logits * temperature: from the gradients of
- * top_w (NULL = 0), scores (NULL = 0), probs (NULL = 0) and of the balance loss
- * over probs (grad_balance, a device scalar, NULL = 0; needs the plan's counts).
- * The bias and the choice get none.  Indices outside the experts are skipped. */
+/* Its gradient with respect to logits: from the gradients of top_w (NULL = 0) and
+ * scores (NULL = 0).  The bias and the choice get none.  Indices outside the
+ * experts are skipped. */
 int qw_moe_route_scored_backward(const float* scores, const int32_t* top_idx, const float* grad_top_w,
-                                 const float* grad_scores, const float* grad_probs, const float* grad_balance,
-                                 const int32_t* counts, int64_t tokens, int64_t experts, int64_t top_k, int score,
-                                 int renormalize, float scale, float temperature, float* grad_logits, void* stream);
+                                 const float* grad_scores, int64_t tokens, int64_t experts, int64_t top_k, int score,
+                                 int renormalize, float scale, float* grad_logits, void* stream);
 
 /* ------------------------------------------------------------------------
  * Microscaled 4-bit floating point.  No reference counterpart (its 4-bit
@@ -528,8 +517,10 @@ int qw_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_
 
 /* out [rows, out_features] = x quantised as above, times the stored matrix
  * [out_features, in_features] transposed: exact products summed in fp32 and
- * rounded once to act_dtype (QW_F32, QW_BF16 or QW_F16, of x and out). */
-size_t qw_mx_matmul_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features);
+ * rounded once to act_dtype (QW_F32, QW_BF16 or QW_F16, of x and out).  A few rows
+ * that start on 16 bytes are read as they lie and need no workspace (0 bytes). */
+size_t qw_mx_matmul_workspace_bytes(const void* x, int act_dtype, int64_t x_row_stride, int64_t rows,
+                                    int64_t out_features, int64_t in_features);
 int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t rows, const void* codes,
                  const void* scales, int64_t out_features, int64_t in_features, void* out, void* workspace,
                  size_t workspace_bytes, void* stream);
@@ -544,19 +535,18 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
 
 /* The SwiGLU experts of qw_moe_experts on microscaled weights and rows:
  *   h = silu(gate_e(x_s)) * up_e(x_s),  y[s] = down_e(h)
- * for s in [kept_offsets[e], kept_offsets[e+1]), x_s = x[row_index[s]] (NULL:
- * x[s]; x has x_rows rows).  x and h are quantised as by qw_mx_quantize (h from
+ * for s in [kept_offsets[e], kept_offsets[e+1]), x_s = x[s] (max_rows rows).  x and h are quantised as by qw_mx_quantize (h from
  * the fp32 sums), products are summed in fp32, y is rounded once to act_dtype.
  * gate, up: stacks [experts, d_ff, d_model]; down: [experts, d_model, d_ff].
  * max_rows bounds kept_offsets[experts]; max_rows_per_expert (0: unknown) only
  * chooses the kernel.  Rows of y past kept_offsets[experts] are left as they were,
  * or become zeros where zero_rest != 0. */
 size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t d_model, int64_t d_ff);
-int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_stride, const int32_t* row_index,
-                  const int32_t* kept_offsets, int64_t experts, int64_t d_model, int64_t d_ff, int64_t max_rows,
-                  int64_t max_rows_per_expert, const void* gate_codes, const void* gate_scales, const void* up_codes,
-                  const void* up_scales, const void* down_codes, const void* down_scales, int zero_rest, void* y,
-                  void* workspace, size_t workspace_bytes, void* stream);
+int qw_mx_experts(const void* x, int act_dtype, int64_t x_row_stride, const int32_t* kept_offsets, int64_t experts,
+                  int64_t d_model, int64_t d_ff, int64_t max_rows, int64_t max_rows_per_expert,
+                  const void* gate_codes, const void* gate_scales, const void* up_codes, const void* up_scales,
+                  const void* down_codes, const void* down_scales, int zero_rest, void* y, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -72,18 +72,16 @@ SIGNATURES = {
     "qw_moe_combine_weighted": (I32, [P, I32, P, P, P, I64, I64, I64, P, I32, P]),
     "qw_moe_combine_backward": (I32, [P, I32, P, I32, P, P, I64, I64, I64, P, P, P]),
     "qw_moe_route_backward": (I32, [P, P, P, P, P, P, P, I64, I64, I64, F32, P, P]),
-    "qw_moe_route_scored": (I32, [P, I32, I64, P, I32, I64, I64, I64, I64, F32, I32, P, I64, I64, I32, I32, F32,
-                                  P, P, P, P, P, P, SZ, P]),
-    "qw_moe_route_scored_from_logits": (I32, [P, I64, I64, I64, I32, P, I64, I64, I32, I32, F32, P, P, P, P, P]),
-    "qw_moe_route_scored_backward": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I32, I32, F32, F32, P, P]),
+    "qw_moe_route_scored_from_logits": (I32, [P, I64, I64, I64, I32, P, I64, I64, I32, I32, F32, P, P, P, P]),
+    "qw_moe_route_scored_backward": (I32, [P, P, P, P, I64, I64, I64, I32, I32, F32, P, P]),
     "qw_mx_quantize": (I32, [P, I32, I64, I64, I64, P, P, P]),
     "qw_mx_dequantize": (I32, [P, P, I64, I64, P, I32, P]),
-    "qw_mx_matmul_workspace_bytes": (SZ, [I64, I64, I64]),
+    "qw_mx_matmul_workspace_bytes": (SZ, [P, I32, I64, I64, I64, I64]),
     "qw_mx_matmul": (I32, [P, I32, I64, I64, P, P, I64, I64, P, P, SZ, P]),
     "qw_mx_matmul_backward_workspace_bytes": (SZ, [I64, I64, I64, I32]),
     "qw_mx_matmul_backward": (I32, [P, I32, I64, P, P, I64, I64, P, P, SZ, P]),
     "qw_mx_experts_workspace_bytes": (SZ, [I64, I64, I64, I64]),
-    "qw_mx_experts": (I32, [P, I32, I64, I64, P, P, I64, I64, I64, I64, I64, P, P, P, P, P, P, I32, P, P, SZ, P]),
+    "qw_mx_experts": (I32, [P, I32, I64, P, I64, I64, I64, I64, I64, P, P, P, P, P, P, I32, P, P, SZ, P]),
 }
 
 _lib: ctypes.CDLL | None = None

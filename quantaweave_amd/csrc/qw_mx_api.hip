@@ -79,8 +79,10 @@ int qw_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_
   return mx_dequantize(codes, scales, rows, cols, out, out_dtype, as_stream(stream));
 }
 
-size_t qw_mx_matmul_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features) {
+size_t qw_mx_matmul_workspace_bytes(const void* x, int act_dtype, int64_t x_row_stride, int64_t rows,
+                                    int64_t out_features, int64_t in_features) {
   if (rows < 1 || out_features < 1 || in_features < 1) return 0;
+  if (mx_few_rows(rows, 1) && mx_rows_takes(x, act_dtype, x_row_stride, in_features)) return 0;
   Carver c(nullptr);
   c.take<char>(static_cast<size_t>(rows) * mx_code_bytes(in_features));
   c.take<char>(static_cast<size_t>(rows) * mx_scale_bytes(in_features));
@@ -100,8 +102,8 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
   QW_REQUIRE(x && out, "x and out are required");
   st = check_matrix(codes, scales, "weight");
   if (st) return st;
-  const size_t need = qw_mx_matmul_workspace_bytes(rows, out_features, in_features);
-  const bool few = mx_few_rows(rows, 1), direct = few && mx_rows_takes(x, act_dtype, x_row_stride, in_features);
+  const size_t need = qw_mx_matmul_workspace_bytes(x, act_dtype, x_row_stride, rows, out_features, in_features);
+  const bool few = mx_few_rows(rows, 1), direct = need == 0;
   if (!direct && (workspace == nullptr || workspace_bytes < need))
     return set_error(QW_ERR_WORKSPACE, "mx_matmul needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
   MxProduct p;
@@ -177,22 +179,19 @@ size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t 
   return c.used + 256;
 }
 
-int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_stride, const int32_t* row_index,
-                  const int32_t* kept_offsets, int64_t experts, int64_t d_model, int64_t d_ff, int64_t max_rows,
-                  int64_t max_rows_per_expert, const void* gate_codes, const void* gate_scales, const void* up_codes,
-                  const void* up_scales, const void* down_codes, const void* down_scales, int zero_rest, void* y,
-                  void* workspace, size_t workspace_bytes, void* stream) {
+int qw_mx_experts(const void* x, int act_dtype, int64_t x_row_stride, const int32_t* kept_offsets, int64_t experts,
+                  int64_t d_model, int64_t d_ff, int64_t max_rows, int64_t max_rows_per_expert,
+                  const void* gate_codes, const void* gate_scales, const void* up_codes, const void* up_scales,
+                  const void* down_codes, const void* down_scales, int zero_rest, void* y, void* workspace,
+                  size_t workspace_bytes, void* stream) {
   clear_error();
   int st = check_act(act_dtype);
   if (st) return st;
   st = check_sizes(max_rows, d_ff, d_model);
   if (st) return st;
   QW_REQUIRE(experts >= 1 && experts <= 65535, "experts out of range: %lld", (long long)experts);
-  QW_REQUIRE(x_rows >= 0 && x_rows <= INT32_MAX / 64, "x_rows out of range: %lld", (long long)x_rows);
-  QW_REQUIRE(row_index != nullptr || x_rows >= max_rows, "x has %lld rows for %lld", (long long)x_rows,
-             (long long)max_rows);
   QW_REQUIRE(x_row_stride >= 0 && max_rows_per_expert >= 0, "strides and bounds must be >= 0");
-  if (max_rows == 0 || x_rows == 0) return QW_OK;
+  if (max_rows == 0) return QW_OK;
   QW_REQUIRE(x && y && kept_offsets, "x, y and kept_offsets are required");
   st = check_matrix(gate_codes, gate_scales, "gate");
   if (!st) st = check_matrix(up_codes, up_scales, "up");
@@ -217,10 +216,9 @@ int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_st
   uint8_t* xs = c.take<uint8_t>(static_cast<size_t>(max_rows) * mx_scale_bytes(d_model));
   if (mx_few_rows(max_rows, experts)) {
     if (mx_rows_takes(x, act_dtype, x_row_stride, d_model)) {
-      p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride, p.row_index = row_index;
+      p.x = x, p.x_dtype = act_dtype, p.x_stride = x_row_stride;
     } else {
-      st = mx_gather(x, act_dtype, max_rows, d_model, x_row_stride, row_index, kept_offsets + experts, xq, xs,
-                     as_stream(stream));
+      st = mx_quantize(x, act_dtype, max_rows, d_model, x_row_stride, xq, xs, as_stream(stream));
       if (st) return st;
       p.x_codes = xq, p.x_scales = xs;
     }
@@ -230,7 +228,7 @@ int qw_mx_experts(const void* x, int act_dtype, int64_t x_rows, int64_t x_row_st
   }
   const int64_t cap = max_rows_per_expert > 0 && max_rows_per_expert < max_rows ? max_rows_per_expert : max_rows;
   MxPrepare prep;
-  prep.row_index = row_index, prep.offsets = kept_offsets, prep.groups = experts;
+  prep.offsets = kept_offsets, prep.groups = experts;
   prep.chunk_rows = p.chunk_rows = d.chunk_rows = mx_group_chunk(max_rows, experts, cap);
   prep.table = c.take<int4>(static_cast<size_t>(mx_max_chunks(max_rows, experts, prep.chunk_rows)) + 1);
   prep.zero_out = zero_rest ? y : nullptr;

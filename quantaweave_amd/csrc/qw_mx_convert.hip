@@ -46,23 +46,19 @@ __device__ __forceinline__ uint32_t block_scale(const MxPiece<DT>& v) {
 template <int DT>
 __global__ __launch_bounds__(kConvertThreads) void mx_quantize_kernel(const void* __restrict__ x, int64_t stride,
                                                                       int cols, uint32_t pieces, int64_t total,
-                                                                      bool aligned, const int32_t* __restrict__ index,
-                                                                      const int32_t* __restrict__ end,
-                                                                      uint32_t* __restrict__ codes,
+                                                                      bool aligned, uint32_t* __restrict__ codes,
                                                                       uint8_t* __restrict__ scales) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvertThreads + threadIdx.x;
   if (i >= total) return;  // whole blocks: total is a multiple of 16 and the four lanes of a block go together
   const int64_t row = total <= INT32_MAX ? static_cast<uint32_t>(i) / pieces : i / pieces;
   const int col = static_cast<int>(i - row * pieces) * 8;
-  if (end != nullptr && row >= *end) return;  // rows that index says nothing of
-  const int64_t src = index != nullptr ? index[row] : row;
-  const MxPiece<DT> v = mx_load_piece<DT>(x, src * stride + col, cols - col, aligned);
+  const MxPiece<DT> v = mx_load_piece<DT>(x, row * stride + col, cols - col, aligned);
   const uint32_t s = block_scale<DT>(v);
   codes[i] = mx_piece_codes<DT>(v, s);
   if (threadIdx.x % 4 == 0) scales[i / 4] = static_cast<uint8_t>(s);
 }
 
-// Rows for the tile kernel: gathered, the scales step by step.  A workgroup holds
+// Rows for the tile kernel, the scales step by step.  A workgroup holds
 // sixteen rows by sixteen lanes, a step of 128 columns, and goes through up to
 // kPrepareSteps of them: the scales of a step are one dword per row, sixteen rows
 // side by side.  The last workgroup makes the chunk table; rows of no group are
@@ -92,12 +88,12 @@ __global__ __launch_bounds__(kConvertThreads) void mx_prepare_kernel(const void*
         }
     return;
   }
-  const int64_t src = prep.row_index != nullptr ? prep.row_index[row] : row;
+  const int64_t base = row * stride;
   MxPiece<DT> v[kPrepareSteps];
 #pragma unroll
   for (int j = 0; j < kPrepareSteps; ++j) {
     const int col = (s0 + j) * kMxStep + piece * 8;
-    v[j] = mx_load_piece<DT>(x, src * stride + col, cols - col, aligned);
+    v[j] = mx_load_piece<DT>(x, base + col, cols - col, aligned);
   }
 #pragma unroll
   for (int j = 0; j < kPrepareSteps; ++j) {
@@ -146,8 +142,8 @@ __global__ __launch_bounds__(kConvertThreads) void mx_dequantize_kernel(const ui
 
 }  // namespace
 
-int mx_gather(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, const int32_t* index,
-              const int32_t* end, void* codes, void* scales, hipStream_t stream) {
+int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
+                hipStream_t stream) {
   const int64_t pieces = mx_padded(cols) / 8, total = rows * pieces;
   if (total == 0) return QW_OK;
   const int64_t blocks = ceil_div(total, kConvertThreads);
@@ -156,19 +152,14 @@ int mx_gather(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stri
   const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * size % 16 == 0;
   auto go = [&](auto kernel) {
     kernel<<<static_cast<unsigned>(blocks), kConvertThreads, 0, stream>>>(
-        x, stride, static_cast<int>(cols), static_cast<uint32_t>(pieces), total, aligned, index,
-        end, static_cast<uint32_t*>(codes), static_cast<uint8_t*>(scales));
+        x, stride, static_cast<int>(cols), static_cast<uint32_t>(pieces), total, aligned,
+        static_cast<uint32_t*>(codes), static_cast<uint8_t*>(scales));
   };
   if (dtype == QW_F32) go(mx_quantize_kernel<QW_F32>);
   else if (dtype == QW_F16) go(mx_quantize_kernel<QW_F16>);
   else go(mx_quantize_kernel<QW_BF16>);
   QW_LAUNCH_CHECK("mx_quantize_kernel");
   return QW_OK;
-}
-
-int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
-                hipStream_t stream) {
-  return mx_gather(x, dtype, rows, cols, stride, nullptr, nullptr, codes, scales, stream);
 }
 
 int mx_prepare(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, uint8_t* codes, uint8_t* scales,

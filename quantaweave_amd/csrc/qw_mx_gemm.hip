@@ -8,17 +8,22 @@
 // per row) through a ring of as many stages as the LDS holds (four at 320 rows,
 // seven at 64).  The ring runs on across tiles: while a tile's last slices are
 // multiplied and its result is stored, the first slices of the next are on their
-// way, so that neither a start nor an epilogue leaves the memory idle (one tile
-// per workgroup, whose slices of 256 columns began anew with each: 16384 rows of
-// 64 experts, d 2048, f 1024, gate and up 65 us, down 51 us, now @GATEUP@ and @DOWN@).
+// way, so that neither a start nor an epilogue leaves the memory idle.  One tile
+// per workgroup, whose slices of 256 columns began anew with each, took for 16384
+// rows of 64 experts (d 2048, f 1024) 65 us for gate and up and 51 us for down, now
+// 65 and 42; for 4099 rows of popular experts (d 4096, f 1408) 149 and 95 us, now
+// 137 and 75; a product of few tiles has nothing to run on into and loses (1023 x
+// 1408 x 4096: 11.3 us, now 14.1).  Bound by the matrix instructions: 8192 x 2048 x
+// 7168 in 80 us, 3.0 PFLOP/s; a slice of 320 rows takes about 2000 cycles of which
+// its instructions issue in 1280.
 // Every wave issues the same number of loads per slice (rows past the end are
 // clamped to a valid row, their results never stored; past the last slice the
 // last one is requested again), so a fixed vmcnt marks a slice as landed.
 //
 // LDS rows are 64 bytes, four 16-byte pieces, each one block of 32 columns; pieces
 // are stored XOR-swizzled so that the sixteen rows that a quarter wave reads cover
-// all banks.  Rows are stored ones in row order (gathered when they were
-// quantised), their scales step by step: dword [step][row].
+// all banks.  Rows are stored ones in row order, their scales step by
+// step: dword [step][row].
 //
 // Waves form a 2 x 4 grid: wave (wm, wn) multiplies row tiles wm, wm + 2, ... (32
 // rows each) by its 64 weight rows, with the instruction of 32 x 32 rows and 64
@@ -342,7 +347,7 @@ __global__ __launch_bounds__(MX_THREADS) void mx_gemm_kernel(
       // 16-bit results go through LDS, a row tile at a time in this wave's part of the
       // stage that the next request will fill (free once every wave is done with the
       // last slice), so that a store is eight whole 128-byte lines (a lane's own 16
-      // bytes of 32 rows each: 320 x 256 results 12 us instead of @EPI@).
+      // bytes of 32 rows each: 320 x 256 results 12 us instead of 3.5 us).
       constexpr int PASSES = MX_WAVES * 32 * 128 <= STAGE ? 1 : 2;  // sixteen rows at a time in small stages
       constexpr int MINE = 32 * 128 / PASSES;
       static_assert(MX_WAVES * MINE <= STAGE, "the rows of every wave fit a stage");

@@ -16,9 +16,8 @@ struct MxMatrix {
 //   one matrix  : out[r] = x[r] . a[n]               [rows, n] of out_dtype
 //   two matrices: h[r] = silu(x[r] . a[n]) * (x[r] . b[n]), stored microscaled:
 //                 h_codes [rows, padded(n) / 2] and h_scales
-// launch_mx_rows takes numbers of x_dtype (x, x_stride; row_index picks the row
-// behind each, NULL: the row itself) or stored rows (x_codes, x_scales), with the
-// scales of stored rows and of h as [rows][padded / 32].
+// launch_mx_rows takes numbers of x_dtype (x, x_stride) or stored rows (x_codes,
+// x_scales), with the scales of stored rows and of h as [rows][padded / 32].
 // launch_mx_gemm takes stored rows in row order, with the scales of rows and of h
 // step by step, [padded / 128][rows][4], and grouped rows as a chunk table:
 // table[0].x chunks, table[1 + i] = {group, first row, rows, 0} of up to chunk_rows.
@@ -28,7 +27,6 @@ struct MxProduct {
   int64_t x_stride = 0;
   const uint8_t* x_codes = nullptr;
   const uint8_t* x_scales = nullptr;
-  const int32_t* row_index = nullptr;
   const int32_t* offsets = nullptr;
   const int4* table = nullptr;
   int chunk_rows = 0;
@@ -58,7 +56,6 @@ inline bool mx_few_rows(int64_t rows, int64_t groups) { return rows <= groups * 
 
 // What launch_mx_gemm's rows need beside quantisation, in the same pass.
 struct MxPrepare {
-  const int32_t* row_index = nullptr;  // gather
   const int32_t* offsets = nullptr;    // grouped rows: the chunk table
   int64_t groups = 0;
   int4* table = nullptr;
@@ -70,9 +67,6 @@ int mx_prepare(const void* x, int dtype, int64_t rows, int64_t cols, int64_t str
 
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
                 hipStream_t stream);
-// The same of the rows x[index[r]] (NULL: x[r]) for r < *end (device; NULL: all).
-int mx_gather(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, const int32_t* index,
-              const int32_t* end, void* codes, void* scales, hipStream_t stream);
 int mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
                   hipStream_t stream);
 

@@ -3,17 +3,16 @@
 //
 // One workgroup owns sixteen rows of a group and 32 columns of the result (two
 // matrices: 32 gate and the matching 32 up columns, one block of the hidden row).
-// The K axis is split over its waves in pairs of steps, 256 columns, so that a
-// wave's two loads of a weight row are one 128-byte line and the pair's scales
-// eight bytes: its lanes hold 16 weight rows by four blocks, one 16-byte load per
-// lane, step and 16 columns of the result.  A pair's loads go out together, with
-// one matrix before the rows are looked at.
-// Rows given as numbers become codes in the registers of the lane that multiplies
-// them, whose 32 numbers are one block.  The partial sums meet in LDS and are added
-// in wave order (the same sum whatever the rows beside it).
+// The K axis is split over its waves in turns of one or two steps of 128 columns:
+// its lanes hold 16 weight rows by four blocks, one 16-byte load per lane, step and
+// 16 columns of the result, and all loads of a turn go out before the first is
+// waited for.  Rows given as numbers become codes in the registers of the lane that
+// multiplies them, whose 32 numbers are one block.  The partial sums meet in LDS and
+// are added in wave order (the same sum whatever the rows beside it).
 //
-// Bound by the weight stream where many experts are touched (@EXPERTS@), by latency
-// for a single matrix (1 row, 2048 x 7168: @ONE@).
+// Bound by the weight stream where many experts are touched: 128 rows of 64 experts,
+// d 2048, f 1024, gate and up 45 us (2.7 TB/s), down 19 us (3.3 TB/s).  Bound by
+// latency for a single matrix (1 row, 2048 x 7168: 5.6 us, 1.4 TB/s).
 #include "qw_mx_product.h"
 
 namespace qw {
@@ -22,15 +21,24 @@ namespace {
 
 constexpr int kRowsM = 16, kRowsN = 32;
 constexpr int kStored = -1;  // XDT of rows that are stored microscaled
-constexpr int kRowsLayers = 2;  // workgroups that share a group's row chunks
+// Steps of 128 columns that a wave takes together.  Two make its two loads of a
+// weight row one 128-byte line (the down product above with one: 24.5 us); two
+// matrices and the numbers of a row leave the registers of two workgroups per unit
+// only one (gate and up above with two, and the next two requested ahead, spilled
+// eighteen registers: 58 us).
+template <int XDT, bool GATEUP>
+constexpr int kRowsSteps = GATEUP && XDT != kStored ? 1 : 2;
+// Workgroups that share a group's row chunks: the grid is fixed before the groups'
+// sizes are known, and a group has sixteen rows at most on average.
+constexpr int kRowsLayers = 2;
 
-// Eight numbers from element i (on 16 bytes), or zeros.
+// Eight numbers from a place on 16 bytes, or zeros.
 template <int DT>
-__device__ __forceinline__ MxPiece<DT> whole_piece(const void* __restrict__ p, int64_t i, bool there) {
+__device__ __forceinline__ MxPiece<DT> whole_piece(const char* __restrict__ p, bool there) {
   MxPiece<DT> r;
   uint4 a = make_uint4(0, 0, 0, 0), b = a;
   if (there) {
-    const uint4* const at = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (DT == QW_F32 ? 4 : 2));
+    const uint4* const at = reinterpret_cast<const uint4*>(p);
     a = at[0];
     if constexpr (DT == QW_F32) b = at[1];
   }
@@ -42,14 +50,10 @@ __device__ __forceinline__ MxPiece<DT> whole_piece(const void* __restrict__ p, i
 template <int XDT, bool GATEUP, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave, 4) void mx_rows_kernel(
     const void* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ x_scales,
-    const int32_t* __restrict__ row_index, const int32_t* __restrict__ offsets, int groups, int rows, MxMatrix wa,
-    MxMatrix wb, int n, int k, int col_tiles, int layers, void* __restrict__ out, int out_dtype, bool zero_rest,
+    const int32_t* __restrict__ offsets, int groups, int rows, MxMatrix wa, MxMatrix wb, int n, int k, int col_tiles, int layers, void* __restrict__ out, int out_dtype, bool zero_rest,
     uint8_t* __restrict__ h_codes, uint8_t* __restrict__ h_scales) {
   constexpr int TILES = GATEUP ? 4 : 2;  // 16 weight rows each: two of gate, two of up
-  constexpr int THREADS = WAVES * kWave;
-  // Two matrices' fragments and the numbers of a row together do not fit the
-  // registers of two workgroups per unit: there the rows come first.
-  constexpr bool kRowsFirst = GATEUP && XDT != kStored;
+  constexpr int THREADS = WAVES * kWave, STEPS = kRowsSteps<XDT, GATEUP>;
   __shared__ f32x4 part[WAVES][TILES][kWave];
   const int ct = blockIdx.x % col_tiles, place = blockIdx.x / col_tiles;
   const int e = offsets ? place % groups : 0, layer = offsets ? place / groups : place;
@@ -63,7 +67,7 @@ __global__ __launch_bounds__(WAVES* kWave, 4) void mx_rows_kernel(
   const int n0 = ct * kRowsN;
   const int64_t pitch = (k + kMxStep - 1) / kMxStep * static_cast<int64_t>(kMxStep);
   const int64_t cb = pitch / 2, sb = pitch / kMxBlock;
-  const int steps = static_cast<int>(pitch / kMxStep), pairs = (steps + 1) / 2;
+  const int steps = static_cast<int>(pitch / kMxStep), turns = (steps + STEPS - 1) / STEPS;
 
   if (!GATEUP && zero_rest && offsets) {  // the rows behind the last group, shared by all workgroups
     for (int64_t r0 = static_cast<int64_t>(max(offsets[groups], 0)) + place * kRowsM; r0 < rows;
@@ -95,34 +99,28 @@ __global__ __launch_bounds__(WAVES* kWave, 4) void mx_rows_kernel(
     f32x4 acc[TILES];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 w[TILES][2];
-    uint32_t ws[TILES][2];
-    // a pair of steps; where the last holds one, the second rereads it and is not multiplied
-    auto load = [&](int p) {
-      const int second = 2 * p + 1 < steps ? 1 : 0;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        const uint8_t* const c = codes[t / 2] + static_cast<int64_t>(p) * 128;
-        const uint8_t* const s = scales[t / 2] + static_cast<int64_t>(p) * 8;
-        w[t][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(c + w_off[t % 2]));
-        w[t][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(c + second * 64 + w_off[t % 2]));
-        ws[t][0] = *reinterpret_cast<const uint32_t*>(s + s_off[t % 2]);
-        ws[t][1] = *reinterpret_cast<const uint32_t*>(s + second * 4 + s_off[t % 2]);
-      }
-    };
-    int first = wave;
-    asm volatile("" : "+s"(first));  // the next chunk loads its weights again: kept, they would cost the registers twice
-    if (!kRowsFirst && first < pairs) load(first);
     // rows past the count repeat the last one; their results are not stored
-    const int64_t rr = r0 + min(l16, count - 1);
-    const int64_t row = row_index ? row_index[rr] : rr;
+    const int64_t row = r0 + min(l16, count - 1);
+    constexpr int kSize = XDT == QW_F32 ? 4 : 2;
+    const char* const x_row = static_cast<const char*>(x) + (row * x_stride + lq * kMxBlock) * kSize;
 #pragma unroll 1
-    for (int p = first; p < pairs; p += WAVES) {
-      u32x4 xc[2];
-      uint32_t xs[2];
+    for (int p = wave; p < turns; p += WAVES) {
+      u32x4 w[TILES][STEPS], xc[STEPS];
+      uint32_t ws[TILES][STEPS], xs[STEPS];
+      // all loads of a turn go out together; where the last turn of two holds one step,
+      // the second rereads it and is not multiplied
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int s = min(2 * p + j, steps - 1);
+      for (int j = 0; j < STEPS; ++j) {
+        const int64_t s = min(STEPS * p + j, steps - 1);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          w[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(codes[t / 2] + s * 64 + w_off[t % 2]));
+          ws[t][j] = *reinterpret_cast<const uint32_t*>(scales[t / 2] + s * 4 + s_off[t % 2]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        const int s = min(STEPS * p + j, steps - 1);
         if constexpr (XDT == kStored) {
           xc[j] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(x) + row * cb + s * 64 + lq * 16);
           xs[j] = x_scales[row * sb + s * 4 + lq];
@@ -130,7 +128,8 @@ __global__ __launch_bounds__(WAVES* kWave, 4) void mx_rows_kernel(
           const int col = s * kMxStep + lq * kMxBlock;
           MxPiece<XDT> v[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] = whole_piece<XDT>(x, row * x_stride + col + 8 * q, col + 8 * q < k);
+          for (int q = 0; q < 4; ++q)
+            v[q] = whole_piece<XDT>(x_row + (s * kMxStep + 8 * q) * kSize, col + 8 * q < k);
           uint32_t top = 0;
 #pragma unroll
           for (int q = 0; q < 4; ++q) top = mx_top_max<XDT>(top, mx_piece_top<XDT>(v[q]));
@@ -139,16 +138,11 @@ __global__ __launch_bounds__(WAVES* kWave, 4) void mx_rows_kernel(
           for (int q = 0; q < 4; ++q) xc[j][q] = mx_piece_codes<XDT>(v[q], xs[j]);
         }
       }
-      if (kRowsFirst) {
-        asm volatile("" ::: "memory");  // the rows' registers are free before the weights' are taken
-        load(p);
-      }
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma(w[t][0], xc[0], acc[t], ws[t][0] >> (8 * lq), xs[0]);
-      if (2 * p + 1 < steps)
+      for (int j = 0; j < STEPS; ++j)
+        if (j == 0 || STEPS * p + j < steps)
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma(w[t][1], xc[1], acc[t], ws[t][1] >> (8 * lq), xs[1]);
-      if (!kRowsFirst && p + WAVES < pairs) load(p + WAVES);
+          for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma(w[t][j], xc[j], acc[t], ws[t][j] >> (8 * lq), xs[j]);
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) part[wave][t][lane] = acc[t];
@@ -205,15 +199,15 @@ int launch_t(const MxProduct& p, hipStream_t stream) {
   const void* x = XDT == kStored ? p.x_codes : p.x;
   auto go = [&](auto kernel, int waves) {
     kernel<<<static_cast<unsigned>(grid), waves * kWave, 0, stream>>>(
-        x, p.x_stride, p.x_scales, p.row_index, p.offsets, static_cast<int>(p.groups),
+        x, p.x_stride, p.x_scales, p.offsets, static_cast<int>(p.groups),
         static_cast<int>(p.rows), p.a, p.b, static_cast<int>(p.n), static_cast<int>(p.k), static_cast<int>(col_tiles),
         static_cast<int>(layers), p.out, p.out_dtype, p.zero_rest, p.h_codes, p.h_scales);
   };
-  // a wave per pair of steps up to eight: more waves than pairs would idle
-  const bool eight = mx_padded(p.k) > 4 * 2 * kMxStep;
-  if (gateup && eight) go(mx_rows_kernel<XDT, true, 8>, 8);
+  // a wave per turn of steps, four or eight: more waves than turns would idle
+  const int64_t steps = mx_padded(p.k) / kMxStep;
+  if (gateup && steps > 4 * kRowsSteps<XDT, true>) go(mx_rows_kernel<XDT, true, 8>, 8);
   else if (gateup) go(mx_rows_kernel<XDT, true, 4>, 4);
-  else if (eight) go(mx_rows_kernel<XDT, false, 8>, 8);
+  else if (steps > 4 * kRowsSteps<XDT, false>) go(mx_rows_kernel<XDT, false, 8>, 8);
   else go(mx_rows_kernel<XDT, false, 4>, 4);
   QW_LAUNCH_CHECK("mx_rows_kernel");
   return QW_OK;

@@ -996,20 +996,6 @@ static int launch_router(const void* x, int xdt, int64_t x_stride, const void* w
                             splits_out, stream, nullptr, 0);
 }
 
-// The router's logits alone, for a choice made elsewhere: into `logits`
-// (*splits = 0), or as *splits partial sums in `partial`.
-int router_logits(const void* x, int xdt, int64_t x_stride, const void* w, int wdt, int64_t T, int64_t D, int64_t E,
-                  float temperature, float* logits, float* partial, size_t partial_bytes, int* splits,
-                  hipStream_t stream) {
-  QW_REQUIRE(xdt == QW_F32 || xdt == QW_BF16 || xdt == QW_F16, "router input dtype must be f32, bf16 or f16");
-  QW_REQUIRE(wdt == QW_F32 || wdt == QW_BF16 || wdt == QW_F16, "router weight dtype must be f32, bf16 or f16");
-  QW_REQUIRE(D >= 1 && D <= INT32_MAX, "d_model out of range");
-  QW_REQUIRE(x_stride >= D, "x row stride %lld smaller than d_model %lld", (long long)x_stride, (long long)D);
-  QW_REQUIRE(temperature > 0.0f, "router_temperature must be positive");
-  QW_REQUIRE(x && w && logits, "x, router_w and logits are required");
-  return launch_router(x, xdt, x_stride, w, wdt, T, D, E, temperature, logits, partial, partial_bytes, splits, stream);
-}
-
 int route(const void* x, int xdt, int64_t x_stride, const void* w, int wdt, int64_t T, int64_t D, int64_t E,
           int64_t K, float temperature, const float* bias, float* logits, float* probs, int32_t* top_idx,
           float* top_w, float* partial, size_t partial_bytes, hipStream_t stream, bool select_logits) {

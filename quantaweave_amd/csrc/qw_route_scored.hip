@@ -17,9 +17,6 @@
 
 namespace qw {
 
-int router_logits(const void* x, int xdt, int64_t x_stride, const void* w, int wdt, int64_t T, int64_t D, int64_t E,
-                  float temperature, float* logits, float* partial, size_t partial_bytes, int* splits,
-                  hipStream_t stream);
 int route_validate(int64_t T, int64_t E, int64_t K);
 
 namespace {
@@ -65,9 +62,8 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // experts share the largest upper half.
 template <int EPL>
 __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_kernel(
-    const float* __restrict__ partial, int splits, float temperature, const float* __restrict__ logits,
-    float* __restrict__ logits_out, int T, int E, int K, const float* __restrict__ bias, ScoredRule rule,
-    float* __restrict__ scores, float* __restrict__ probs, int32_t* __restrict__ top_idx, float* __restrict__ top_w) {
+    const float* __restrict__ logits, int T, int E, int K, const float* __restrict__ bias, ScoredRule rule,
+    float* __restrict__ scores, int32_t* __restrict__ top_idx, float* __restrict__ top_w) {
   __shared__ double choice[kRouteWaves][EPL * kWave];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int t = blockIdx.x * kRouteWaves + wave;
@@ -78,17 +74,7 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_kernel(
 #pragma unroll
   for (int c = 0; c < EPL; ++c) {
     const int e = lane * EPL + c;
-    l[c] = -__builtin_inff();
-    if (e < E) {
-      if (partial != nullptr) {
-        float v = partial[base + e];
-        for (int sp = 1; sp < splits; ++sp) v += partial[static_cast<int64_t>(sp) * T * E + base + e];
-        l[c] = v / temperature;
-        logits_out[base + e] = l[c];
-      } else {
-        l[c] = logits[base + e];
-      }
-    }
+    l[c] = e < E ? logits[base + e] : -__builtin_inff();
     nan |= l[c] != l[c];
   }
   // ---- scores ----
@@ -120,15 +106,6 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_kernel(
     sel[c] = s[c] + (bias != nullptr && e < E ? static_cast<double>(bias[e]) : 0.0);
     if (sel[c] != sel[c] || e >= E) sel[c] = -__builtin_inf();
     if (e < E) scores[base + e] = static_cast<float>(s[c]);
-  }
-  if (probs != nullptr) {
-    double sum = 0.0;
-#pragma unroll
-    for (int c = 0; c < EPL; ++c) sum += s[c];
-    sum = wave_sum_d(sum);
-#pragma unroll
-    for (int c = 0; c < EPL; ++c)
-      if (lane * EPL + c < E) probs[base + lane * EPL + c] = sum > 0.0 || sum != sum ? static_cast<float>(s[c] / sum) : 0.0f;
   }
   // ---- the groups that stay ----
   uint32_t hi[EPL], lo[EPL];
@@ -232,19 +209,15 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_kernel(
   }
 }
 
-// One wave per token.  With g the gradient of w, P = s / sum(s) (sigmoid scores
-// normalised; softmax scores are their own), and idx_j the choices:
+// One wave per token.  With g the gradient of w and idx_j the choices:
 //   dp_j  = scale * (g_j - sum_i g_i s_idx_i / S) / S   (S the renormalising sum; scale * g_j without)
-//   dP_e  = grad_probs_e + grad_balance * E * counts_e / (T * K * T)
-//   ds_e  = grad_scores_e + sum_{idx_j = e} dp_j + (softmax: dP_e; sigmoid: (dP_e - sum dP P) / sum(s))
+//   ds_e  = grad_scores_e + sum_{idx_j = e} dp_j
 //   dl_e  = softmax: s_e (ds_e - sum ds s);  sigmoid: ds_e s_e (1 - s_e)
 // An index outside [0, E) is skipped.
 template <int EPL>
 __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_backward_kernel(
     const float* __restrict__ scores, const int32_t* __restrict__ top_idx, const float* __restrict__ grad_top_w,
-    const float* __restrict__ grad_scores, const float* __restrict__ grad_probs,
-    const float* __restrict__ grad_balance, const int32_t* __restrict__ counts, int T, int E, int K, ScoredRule rule,
-    float temperature, float* __restrict__ out) {
+    const float* __restrict__ grad_scores, int T, int E, int K, ScoredRule rule, float* __restrict__ out) {
   const int lane = threadIdx.x % kWave;
   const int t = blockIdx.x * kRouteWaves + threadIdx.x / kWave;
   if (t >= T) return;
@@ -264,22 +237,12 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_backward_kern
     const float S = wave_sum_f(pj) + static_cast<float>(kRouteEps);
     dpj = (gj - wave_sum_f(gj * pj) / S) / S;
   }
-  const float bal = grad_balance ? grad_balance[0] * static_cast<float>(E) /
-                                       (static_cast<float>(T) * static_cast<float>(K) * static_cast<float>(T))
-                                 : 0.0f;
-  const bool normal = (grad_probs != nullptr || grad_balance != nullptr);
-  float s[EPL], ds[EPL], dP[EPL];
-  float sum = 0.0f, dot = 0.0f;
+  float s[EPL], ds[EPL];
 #pragma unroll
   for (int c = 0; c < EPL; ++c) {
     const int e = lane * EPL + c;
     s[c] = e < E ? scores[base + e] : 0.0f;
     ds[c] = e < E && grad_scores ? grad_scores[base + e] : 0.0f;
-    dP[c] = 0.0f;
-    if (e < E && grad_probs) dP[c] += grad_probs[base + e];
-    if (e < E && grad_balance) dP[c] += bal * static_cast<float>(counts[e]);
-    sum += s[c];
-    dot = __builtin_fmaf(dP[c], s[c], dot);
   }
   for (int j = 0; j < K; ++j) {
     const int e = __builtin_amdgcn_readlane(idx, j);
@@ -287,16 +250,6 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_backward_kern
 #pragma unroll
     for (int c = 0; c < EPL; ++c)
       if (lane * EPL + c == e) ds[c] += d;
-  }
-  if (normal && rule.softmax) {
-#pragma unroll
-    for (int c = 0; c < EPL; ++c) ds[c] += dP[c];
-  } else if (normal) {
-    sum = wave_sum_f(sum);
-    dot = wave_sum_f(dot);
-    if (sum != 0.0f)
-#pragma unroll
-      for (int c = 0; c < EPL; ++c) ds[c] += (dP[c] - dot / sum) / sum;
   }
   if (rule.softmax) {
     float d = 0.0f;
@@ -312,7 +265,7 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_backward_kern
 #pragma unroll
   for (int c = 0; c < EPL; ++c) {
     const int e = lane * EPL + c;
-    if (e < E) out[base + e] = ds[c] / temperature;
+    if (e < E) out[base + e] = ds[c];
   }
 }
 
@@ -335,18 +288,17 @@ int check_rule(int64_t T, int64_t E, int64_t K, int score, int64_t groups, int64
 
 }  // namespace
 
-int route_scored(const float* partial, int splits, float temperature, const float* logits, float* logits_out,
-                 int64_t T, int64_t E, int64_t K, int score, const float* bias, int64_t groups, int64_t top_groups,
-                 int group_top, int renormalize, float scale, float* scores, float* probs, int32_t* top_idx,
+int route_scored(const float* logits, int64_t T, int64_t E, int64_t K, int score, const float* bias, int64_t groups,
+                 int64_t top_groups, int group_top, int renormalize, float scale, float* scores, int32_t* top_idx,
                  float* top_w, hipStream_t stream) {
   const unsigned grid = static_cast<unsigned>(ceil_div(T, kRouteWaves));
   const ScoredRule rule{score == 0, static_cast<int>(groups), static_cast<int>(top_groups), group_top, renormalize,
                         scale};
   const int t = static_cast<int>(T), e = static_cast<int>(E), k = static_cast<int>(K);
   const int epl = static_cast<int>(ceil_div(E, kWave));
-#define QW_RS(N)                                                                                                    \
-  route_scored_kernel<N><<<grid, kRouteWaves * kWave, 0, stream>>>(partial, splits, temperature, logits, logits_out, t, \
-                                                                   e, k, bias, rule, scores, probs, top_idx, top_w)
+#define QW_RS(N)                                                                                                 \
+  route_scored_kernel<N><<<grid, kRouteWaves * kWave, 0, stream>>>(logits, t, e, k, bias, rule, scores, top_idx, \
+                                                                   top_w)
   if (epl <= 1) QW_RS(1);
   else if (epl <= 2) QW_RS(2);
   else if (epl <= 4) QW_RS(4);
@@ -358,16 +310,15 @@ int route_scored(const float* partial, int splits, float temperature, const floa
 }
 
 int route_scored_backward(const float* scores, const int32_t* top_idx, const float* grad_top_w,
-                          const float* grad_scores, const float* grad_probs, const float* grad_balance,
-                          const int32_t* counts, int64_t T, int64_t E, int64_t K, int score, int renormalize,
-                          float scale, float temperature, float* out, hipStream_t stream) {
+                          const float* grad_scores, int64_t T, int64_t E, int64_t K, int score, int renormalize,
+                          float scale, float* out, hipStream_t stream) {
   const unsigned grid = static_cast<unsigned>(ceil_div(T, kRouteWaves));
   const ScoredRule rule{score == 0, 1, 1, 1, renormalize, scale};
   const int t = static_cast<int>(T), e = static_cast<int>(E), k = static_cast<int>(K);
   const int epl = static_cast<int>(ceil_div(E, kWave));
-#define QW_RS(N)                                                                                                  \
-  route_scored_backward_kernel<N><<<grid, kRouteWaves * kWave, 0, stream>>>(                                      \
-      scores, top_idx, grad_top_w, grad_scores, grad_probs, grad_balance, counts, t, e, k, rule, temperature, out)
+#define QW_RS(N)                                                                                             \
+  route_scored_backward_kernel<N><<<grid, kRouteWaves * kWave, 0, stream>>>(scores, top_idx, grad_top_w,     \
+                                                                            grad_scores, t, e, k, rule, out)
   if (epl <= 1) QW_RS(1);
   else if (epl <= 2) QW_RS(2);
   else if (epl <= 4) QW_RS(4);
@@ -386,51 +337,28 @@ extern "C" {
 
 int qw_moe_route_scored_from_logits(const float* logits, int64_t tokens, int64_t experts, int64_t top_k, int score,
                                     const float* bias, int64_t groups, int64_t top_groups, int group_top,
-                                    int renormalize, float scale, float* scores, float* probs, int32_t* top_idx,
-                                    float* top_w, void* stream) {
+                                    int renormalize, float scale, float* scores, int32_t* top_idx, float* top_w,
+                                    void* stream) {
   clear_error();
   const int st = check_rule(tokens, experts, top_k, score, groups, top_groups, group_top, scale);
   if (st) return st;
   if (tokens == 0) return QW_OK;
   QW_REQUIRE(logits && scores && top_idx && top_w, "logits, scores, top_idx and top_w are required");
-  return route_scored(nullptr, 0, 1.0f, logits, nullptr, tokens, experts, top_k, score, bias, groups, top_groups,
-                      group_top, renormalize, scale, scores, probs, top_idx, top_w, as_stream(stream));
-}
-
-int qw_moe_route_scored(const void* x, int x_dtype, int64_t x_row_stride, const void* router_w, int w_dtype,
-                        int64_t tokens, int64_t d_model, int64_t experts, int64_t top_k, float temperature, int score,
-                        const float* bias, int64_t groups, int64_t top_groups, int group_top, int renormalize,
-                        float scale, float* logits, float* scores, float* probs, int32_t* top_idx, float* top_w,
-                        void* workspace, size_t workspace_bytes, void* stream) {
-  clear_error();
-  int st = check_rule(tokens, experts, top_k, score, groups, top_groups, group_top, scale);
-  if (st) return st;
-  if (tokens == 0) return QW_OK;
-  QW_REQUIRE(scores && top_idx && top_w, "scores, top_idx and top_w are required");
-  int splits = 0;
-  st = router_logits(x, x_dtype, x_row_stride, router_w, w_dtype, tokens, d_model, experts, temperature, logits,
-                     static_cast<float*>(workspace), workspace_bytes, &splits, as_stream(stream));
-  if (st) return st;
-  return route_scored(splits ? static_cast<const float*>(workspace) : nullptr, splits, temperature, logits, logits,
-                      tokens, experts, top_k, score, bias, groups, top_groups, group_top, renormalize, scale, scores,
-                      probs, top_idx, top_w, as_stream(stream));
+  return route_scored(logits, tokens, experts, top_k, score, bias, groups, top_groups, group_top, renormalize, scale,
+                      scores, top_idx, top_w, as_stream(stream));
 }
 
 int qw_moe_route_scored_backward(const float* scores, const int32_t* top_idx, const float* grad_top_w,
-                                 const float* grad_scores, const float* grad_probs, const float* grad_balance,
-                                 const int32_t* counts, int64_t tokens, int64_t experts, int64_t top_k, int score,
-                                 int renormalize, float scale, float temperature, float* grad_logits, void* stream) {
+                                 const float* grad_scores, int64_t tokens, int64_t experts, int64_t top_k, int score,
+                                 int renormalize, float scale, float* grad_logits, void* stream) {
   clear_error();
   const int st = check_rule(tokens, experts, top_k, score, 1, 1, 1, scale);
   if (st) return st;
-  QW_REQUIRE(temperature > 0.0f, "temperature must be positive");
   if (tokens == 0) return QW_OK;
   QW_REQUIRE(scores && grad_logits, "scores and grad_logits are required");
   QW_REQUIRE(grad_top_w == nullptr || top_idx != nullptr, "grad_top_w needs top_idx");
-  QW_REQUIRE(grad_balance == nullptr || counts != nullptr, "grad_balance needs counts");
-  return route_scored_backward(scores, top_idx, grad_top_w, grad_scores, grad_probs, grad_balance, counts, tokens,
-                               experts, top_k, score, renormalize, scale, temperature, grad_logits,
-                               as_stream(stream));
+  return route_scored_backward(scores, top_idx, grad_top_w, grad_scores, tokens, experts, top_k, score, renormalize,
+                               scale, grad_logits, as_stream(stream));
 }
 
 }  // extern "C"

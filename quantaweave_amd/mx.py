@@ -37,22 +37,34 @@ def _rows(x: Tensor, what: str) -> tuple[Tensor, int]:
     """x as [rows, cols] with unit column stride (a view where its strides allow), and its row stride."""
     if x.dim() < 1 or x.size(-1) < 1:
         raise ValueError(f"{what}: rows of at least one column are needed, got shape {tuple(x.shape)}")
-    flat = x.detach().reshape(-1, x.size(-1))
-    if (flat.stride(1) != 1 and flat.size(1) > 1) or flat.stride(0) < 0:
+    if x.requires_grad:
+        x = x.detach()
+    flat = x if x.dim() == 2 else x.reshape(-1, x.size(-1))
+    rows, cols = flat.shape
+    step, unit = flat.stride()
+    if unit != 1 and cols > 1 or step < 0:
         flat = flat.contiguous()
-    return flat, flat.stride(0) if flat.size(0) > 1 else flat.size(1)
+        step = cols
+    return flat, step if rows > 1 else cols
+
+
+def _device(x: Tensor, what: str) -> torch.device:
+    if not x.is_cuda:
+        _hip.require_device(x, what)
+    return x.device
 
 
 def _stored(codes: Tensor, scales: Tensor, dims: int, cols: int, device: torch.device, what: str) -> tuple[Tensor, Tensor]:
     """Checks a stored matrix (or stack): shapes, types, device; contiguous and aligned for the kernels."""
     p = padded_cols(cols)
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise ValueError(f"{what}: codes and scales are uint8, got {codes.dtype} and {scales.dtype}")
-    if codes.dim() != dims or codes.size(-1) != p // 2:
+    shape, of = codes.shape, scales.shape
+    if len(shape) != dims or shape[-1] != p // 2:
         raise ValueError(f"{what}: codes of {cols} columns have {dims} dimensions and {p // 2} bytes a row, "
-                         f"got shape {tuple(codes.shape)}")
-    if tuple(scales.shape) != (*codes.shape[:-1], p // BLOCK):
-        raise ValueError(f"{what}: scales have shape {(*codes.shape[:-1], p // BLOCK)}, got {tuple(scales.shape)}")
+                         f"got shape {tuple(shape)}")
+    if len(of) != dims or of[-1] != p // BLOCK or of[:-1] != shape[:-1]:
+        raise ValueError(f"{what}: scales have shape {(*shape[:-1], p // BLOCK)}, got {tuple(of)}")
     if codes.device != device or scales.device != device:
         raise ValueError(f"{what}: codes and scales must be on {device}")
     codes, scales = codes.contiguous(), scales.contiguous()
@@ -69,43 +81,44 @@ def mx_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     Per block: scale 2^(floor(log2 max|x|) - 2), at least 2^-127; x / scale
     rounded to the nearest code, ties to the even one, saturating at 6.  A
     block holding an infinity or a NaN becomes NaN.  Not differentiable."""
-    _hip.require_device(x, "mx_quantize")
+    dev = _device(x, "mx_quantize")
     act = _hip.act_code(x, "mx_quantize")
     flat, stride = _rows(x, "mx_quantize")
-    cols = flat.size(1)
+    rows, cols = flat.shape
     p = padded_cols(cols)
-    codes = torch.empty(*x.shape[:-1], p // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*x.shape[:-1], p // BLOCK, dtype=torch.uint8, device=x.device)
-    if flat.size(0):
-        _hip.call_on(x.device, "qw_mx_quantize", _hip.ptr(flat), act, flat.size(0), cols, stride, _hip.ptr(codes),
-                     _hip.ptr(scales), _hip.stream(x.device))
+    codes = torch.empty((*x.shape[:-1], p // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*x.shape[:-1], p // BLOCK), dtype=torch.uint8, device=dev)
+    if rows:
+        _hip.call_on(dev, "qw_mx_quantize", _hip.ptr(flat), act, rows, cols, stride, _hip.ptr(codes),
+                     _hip.ptr(scales), _hip.raw_stream(dev))
     return codes, scales
 
 
 def mx_dequantize(codes: Tensor, scales: Tensor, cols: int, dtype: torch.dtype = torch.float32) -> Tensor:
     """The values [..., cols] that codes and scales stand for, rounded once to `dtype`."""
-    _hip.require_device(codes, "mx_dequantize")
-    if cols < 1:
-        raise ValueError(f"mx_dequantize: cols must be positive, got {cols}")
-    codes, scales = _stored(codes, scales, codes.dim(), cols, codes.device, "mx_dequantize")
-    out = torch.empty(*codes.shape[:-1], cols, dtype=dtype, device=codes.device)
+    dev = _device(codes, "mx_dequantize")
+    if cols < 1 or codes.dim() < 1:
+        raise ValueError(f"mx_dequantize: cols must be positive, got {cols} and codes of shape {tuple(codes.shape)}")
+    codes, scales = _stored(codes, scales, codes.dim(), cols, dev, "mx_dequantize")
+    out = torch.empty((*codes.shape[:-1], cols), dtype=dtype, device=dev)
     act = _hip.act_code(out, "mx_dequantize")
     rows = codes.numel() // codes.size(-1)
     if rows:
-        _hip.call_on(codes.device, "qw_mx_dequantize", _hip.ptr(codes), _hip.ptr(scales), rows, cols, _hip.ptr(out),
-                     act, _hip.stream(codes.device))
+        _hip.call_on(dev, "qw_mx_dequantize", _hip.ptr(codes), _hip.ptr(scales), rows, cols, _hip.ptr(out),
+                     act, _hip.raw_stream(dev))
     return out
 
 
 def _matmul(flat: Tensor, stride: int, codes: Tensor, scales: Tensor) -> Tensor:
-    rows, k, n = flat.size(0), flat.size(1), codes.size(0)
-    out = torch.empty(rows, n, dtype=flat.dtype, device=flat.device)
+    (rows, k), n = flat.shape, codes.size(0)
+    dev = flat.device
+    out = torch.empty((rows, n), dtype=flat.dtype, device=dev)
     if rows and n:
-        nbytes = _lib.load().qw_mx_matmul_workspace_bytes(rows, n, k)
-        ws = _hip.workspace(nbytes, flat.device) if nbytes else None
-        _hip.call_on(flat.device, "qw_mx_matmul", _hip.ptr(flat), _hip.act_code(flat, "mx_matmul"), stride, rows,
-                     _hip.ptr(codes), _hip.ptr(scales), n, k, _hip.ptr(out), _hip.ptr(ws), nbytes,
-                     _hip.stream(flat.device))
+        act, at = _hip.act_code(flat, "mx_matmul"), _hip.ptr(flat)
+        nbytes = _lib.load().qw_mx_matmul_workspace_bytes(at, act, stride, rows, n, k)
+        ws = _hip.workspace(nbytes, dev) if nbytes else None
+        _hip.call_on(dev, "qw_mx_matmul", at, act, stride, rows, _hip.ptr(codes), _hip.ptr(scales), n, k,
+                     _hip.ptr(out), _hip.ptr(ws), nbytes, _hip.raw_stream(dev))
     return out
 
 
@@ -134,7 +147,7 @@ class _MxMatmul(torch.autograd.Function):
             nbytes = _lib.load().qw_mx_matmul_backward_workspace_bytes(rows, n, k, act)
             ws = _hip.workspace(nbytes, grad.device)
             _hip.call_on(grad.device, "qw_mx_matmul_backward", _hip.ptr(grad), act, rows, _hip.ptr(codes),
-                         _hip.ptr(scales), n, k, _hip.ptr(gx), _hip.ptr(ws), nbytes, _hip.stream(grad.device))
+                         _hip.ptr(scales), n, k, _hip.ptr(gx), _hip.ptr(ws), nbytes, _hip.raw_stream(grad.device))
         else:
             gx.zero_()
         return gx, None, None
@@ -145,18 +158,17 @@ def mx_matmul(x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
 
     x (float32, bfloat16 or float16) is quantised on the way; the sum is fp32,
     rounded once.  Differentiable in x (the stored matrix takes no gradient)."""
-    _hip.require_device(x, "mx_matmul")
+    dev = _device(x, "mx_matmul")
     _hip.act_code(x, "mx_matmul")
     if x.dim() < 1 or x.size(-1) < 1:
         raise ValueError(f"mx_matmul: rows of at least one column are needed, got shape {tuple(x.shape)}")
-    codes, scales = _stored(codes, scales, 2, x.size(-1), x.device, "mx_matmul")
-    lead = x.shape[:-1]
+    codes, scales = _stored(codes, scales, 2, x.size(-1), dev, "mx_matmul")
     if x.requires_grad and torch.is_grad_enabled():
         _hip.note_stream(x, "mx_matmul")
         out = _MxMatmul.apply(x.reshape(-1, x.size(-1)), codes, scales)
     else:
         out = _matmul(*_rows(x, "mx_matmul"), codes, scales)
-    return out.view(*lead, codes.size(0))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], codes.size(0))
 
 
 def mx_grouped_swiglu(x: Tensor, gate: tuple, up: tuple, down: tuple, offsets: Tensor,
@@ -170,7 +182,7 @@ def mx_grouped_swiglu(x: Tensor, gate: tuple, up: tuple, down: tuple, offsets: T
     silu(gate) * up are quantised on the way, sums are fp32, the result is
     rounded once to x's type.  Not differentiable."""
     what = "mx_grouped_swiglu"
-    _hip.require_device(x, what)
+    _device(x, what)
     act = _hip.act_code(x, what)
     if x.dim() != 2 or x.size(1) < 1:
         raise ValueError(f"{what}: x is [rows, d], got shape {tuple(x.shape)}")
@@ -195,8 +207,8 @@ def mx_grouped_swiglu(x: Tensor, gate: tuple, up: tuple, down: tuple, offsets: T
         offsets = offsets.contiguous()
         nbytes = _lib.load().qw_mx_experts_workspace_bytes(rows, experts, d, ffn)
         ws = _hip.workspace(nbytes, x.device)
-        _hip.call_on(x.device, "qw_mx_experts", _hip.ptr(flat), act, rows, stride, None, _hip.ptr(offsets), experts, d,
-                     ffn, rows, min(max_rows or 0, rows), _hip.ptr(gate[0]), _hip.ptr(gate[1]), _hip.ptr(up[0]),
+        _hip.call_on(x.device, "qw_mx_experts", _hip.ptr(flat), act, stride, _hip.ptr(offsets), experts, d, ffn, rows,
+                     min(max_rows or 0, rows), _hip.ptr(gate[0]), _hip.ptr(gate[1]), _hip.ptr(up[0]),
                      _hip.ptr(up[1]), _hip.ptr(down[0]), _hip.ptr(down[1]), 1, _hip.ptr(out), _hip.ptr(ws), nbytes,
-                     _hip.stream(x.device))
+                     _hip.raw_stream(x.device))
     return out

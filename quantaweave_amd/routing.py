@@ -9,6 +9,7 @@ experts, whose choice is limited to a few groups and balanced by a bias.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -21,9 +22,10 @@ GROUP_SCORES = {"max": 1, "top2": 2}
 MAX_TOP_K = 64
 
 
+@lru_cache(maxsize=256)
 def check_rule(experts: int, top_k: int, score: str, groups: int, top_groups: int, group_score: str,
                scale: float) -> None:
-    """Raises ValueError for a routing rule that no kernel takes."""
+    """Raises ValueError for a routing rule that no kernel takes (one that some kernel takes is looked at once)."""
     if score not in SCORES:
         raise ValueError(f"score must be softmax or sigmoid, got {score!r}")
     if group_score not in GROUP_SCORES:
@@ -60,8 +62,7 @@ class _RouteExperts(torch.autograd.Function):
             dw = None if d_weight is None else d_weight.float().contiguous()
             ds = None if d_scores is None else d_scores.float().contiguous()
             _hip.call_on(scores.device, "qw_moe_route_scored_backward", _hip.ptr(scores), _hip.ptr(index), _hip.ptr(dw),
-                         _hip.ptr(ds), None, None, None, t, e, top_k, SCORES[score], int(renormalize), scale, 1.0,
-                         _hip.ptr(out), _hip.stream(scores.device))
+                         _hip.ptr(ds), t, e, top_k, SCORES[score], int(renormalize), scale, _hip.ptr(out), _hip.raw_stream(scores.device))
         return out, None
 
 
@@ -71,12 +72,12 @@ def _route(logits: Tensor, top_k: int, score: str, bias: Optional[Tensor], group
     dev = logits.device
     logits = logits.contiguous()
     scores = torch.empty_like(logits)
-    index = torch.empty(t, top_k, dtype=torch.int32, device=dev)
-    weight = torch.empty(t, top_k, dtype=torch.float32, device=dev)
+    index = torch.empty((t, top_k), dtype=torch.int32, device=dev)
+    weight = torch.empty((t, top_k), dtype=torch.float32, device=dev)
     if t:
         _hip.call_on(dev, "qw_moe_route_scored_from_logits", _hip.ptr(logits), t, e, top_k, SCORES[score],
                      _hip.ptr(bias), groups, top_groups, GROUP_SCORES[group_score], int(renormalize), scale,
-                     _hip.ptr(scores), None, _hip.ptr(index), _hip.ptr(weight), _hip.stream(dev))
+                     _hip.ptr(scores), _hip.ptr(index), _hip.ptr(weight), _hip.raw_stream(dev))
     return index, weight, scores
 
 
@@ -98,7 +99,8 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
       times `scale`.
 
     Differentiable in logits through weight and scores."""
-    _hip.require_device(logits, "route_experts")
+    if not logits.is_cuda:
+        _hip.require_device(logits, "route_experts")
     if logits.dtype != torch.float32 or logits.dim() < 1:
         raise ValueError(f"route_experts: logits are float32 [..., experts], got {logits.dtype} {tuple(logits.shape)}")
     experts = logits.size(-1)
@@ -108,12 +110,14 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
         if tuple(bias.shape) != (experts,) or bias.device != logits.device:
             raise ValueError(f"route_experts: bias is [{experts}] on {logits.device}")
         bias = bias.detach().float().contiguous()
-    lead = logits.shape[:-1]
-    flat = logits.reshape(-1, experts)
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, experts)
     rule = (top_k, score, bias, groups, top_groups, group_score, bool(renormalize), float(scale))
     if logits.requires_grad and torch.is_grad_enabled():
         _hip.note_stream(logits, "route_experts")
         index, weight, scores = _RouteExperts.apply(flat, rule)
     else:
         index, weight, scores = _route(flat.detach(), *rule)
+    if logits.dim() == 2:
+        return index, weight, scores
+    lead = logits.shape[:-1]
     return index.view(*lead, top_k), weight.view(*lead, top_k), scores.view(*lead, experts)

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import quantaweave_amd as qa
+from quantaweave_amd import _hip, _lib
 from tests import mx_oracle as ref
 
 pytestmark = pytest.mark.gpu
@@ -212,6 +213,22 @@ def test_grouped_swiglu_rows_past_the_last_group_are_zero():
     got = qa.mx_grouped_swiglu(x.cuda(), cuda(gate), cuda(up), cuda(down), offsets.cuda())
     close(got, want, ref.allowed(want, err, torch.bfloat16))
     assert not got[77:].any()
+
+
+@pytest.mark.parametrize("tail", [12, 200])  # few rows per expert, and the tiles
+@pytest.mark.parametrize("zero", [0, 1])
+def test_experts_entry_point_leaves_or_clears_the_rows_behind_the_last_group(tail, zero):
+    x, gate, up, down, offsets, want, err = grouped(gen(9), [5, 0, 30, 2], 256, 128, torch.bfloat16, tail=tail)
+    rows, x = x.size(0), x.cuda()
+    y = torch.full((rows, 256), 7.0, dtype=torch.bfloat16, device="cuda")
+    m = [t for pair in (gate, up, down) for t in cuda(pair)]
+    offsets = offsets.cuda()
+    nbytes = _lib.load().qw_mx_experts_workspace_bytes(rows, 4, 256, 128)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    _lib.call("qw_mx_experts", _hip.ptr(x), _lib.QW_BF16, 256, _hip.ptr(offsets), 4, 256, 128, rows, 30,
+              *(_hip.ptr(t) for t in m), zero, _hip.ptr(y), _hip.ptr(ws), nbytes, _hip.stream(x.device))
+    close(y[:37], want[:37], ref.allowed(want[:37], err[:37], torch.bfloat16))
+    assert (y[37:] == (0.0 if zero else 7.0)).all()
 
 
 def test_grouped_swiglu_without_rows():

@@ -39,17 +39,15 @@ def test_entry_points_check_their_arguments_before_any_launch():
         assert status == _lib.QW_ERR_INVALID and word in lib.qw_last_error(), lib.qw_last_error()
 
     route = lib.qw_moe_route_scored_from_logits
-    refused(route(one, 4, 64, 65, 0, None, 1, 1, 2, 1, 1.0, one, None, one, one, None), b"top_k")
-    refused(route(one, 4, 64, 2, 2, None, 1, 1, 2, 1, 1.0, one, None, one, one, None), b"score")
-    refused(route(one, 4, 64, 2, 0, None, 7, 1, 2, 1, 1.0, one, None, one, one, None), b"groups")
-    refused(route(one, 4, 64, 2, 0, None, 8, 9, 2, 1, 1.0, one, None, one, one, None), b"top_groups")
-    refused(route(one, 4, 64, 9, 0, None, 8, 1, 2, 1, 1.0, one, None, one, one, None), b"top_k")
-    refused(route(one, 4, 64, 2, 0, None, 8, 1, 3, 1, 1.0, one, None, one, one, None), b"group_top")
-    refused(route(None, 4, 64, 2, 0, None, 8, 1, 2, 1, 1.0, one, None, one, one, None), b"logits")
-    refused(lib.qw_moe_route_scored_backward(one, one, one, None, None, one, None, 4, 8, 2, 0, 1, 1.0, 1.0, one, None),
-            b"counts")
-    refused(lib.qw_moe_route_scored_backward(one, one, one, None, None, None, None, 4, 8, 2, 0, 1, 1.0, 0.0, one, None),
-            b"temperature")
+    refused(route(one, 4, 64, 65, 0, None, 1, 1, 2, 1, 1.0, one, one, one, None), b"top_k")
+    refused(route(one, 4, 64, 2, 2, None, 1, 1, 2, 1, 1.0, one, one, one, None), b"score")
+    refused(route(one, 4, 64, 2, 0, None, 7, 1, 2, 1, 1.0, one, one, one, None), b"groups")
+    refused(route(one, 4, 64, 2, 0, None, 8, 9, 2, 1, 1.0, one, one, one, None), b"top_groups")
+    refused(route(one, 4, 64, 9, 0, None, 8, 1, 2, 1, 1.0, one, one, one, None), b"top_k")
+    refused(route(one, 4, 64, 2, 0, None, 8, 1, 3, 1, 1.0, one, one, one, None), b"group_top")
+    refused(route(None, 4, 64, 2, 0, None, 8, 1, 2, 1, 1.0, one, one, one, None), b"logits")
+    refused(lib.qw_moe_route_scored_backward(one, None, one, None, 4, 8, 2, 0, 1, 1.0, one, None), b"top_idx")
+    refused(lib.qw_moe_route_scored_backward(None, one, one, None, 4, 8, 2, 0, 1, 1.0, one, None), b"scores")
     refused(lib.qw_mx_quantize(one, 7, 4, 64, 64, one, one, None), b"dtype")
     refused(lib.qw_mx_quantize(one, 0, 4, 0, 64, one, one, None), b"cols")
     refused(lib.qw_mx_quantize(one, 0, 4, 64, -1, one, one, None), b"stride")
@@ -57,18 +55,18 @@ def test_entry_points_check_their_arguments_before_any_launch():
     refused(lib.qw_mx_dequantize(one, 66, 4, 64, one, 0, None), b"on 4")
     refused(lib.qw_mx_matmul(one, 1, 64, 4, None, one, 8, 64, one, None, 0, None), b"weight")
     refused(lib.qw_mx_matmul(one, 1, 64, -1, one, one, 8, 64, one, None, 0, None), b"rows")
-    refused(lib.qw_mx_experts(one, 1, 3, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, 0, one, one, 1 << 30,
-                              None), b"rows")
-    refused(lib.qw_mx_experts(one, 1, 4, 64, None, one, 0, 64, 64, 4, 0, one, one, one, one, one, one, 0, one, one, 1 << 30,
-                              None), b"experts")
+    weights = [one] * 6
+    refused(lib.qw_mx_experts(one, 1, 64, one, 2, 64, 64, -1, 0, *weights, 0, one, one, 1 << 30, None), b"rows")
+    refused(lib.qw_mx_experts(one, 1, -64, one, 2, 64, 64, 4, 0, *weights, 0, one, one, 1 << 30, None), b"strides")
+    refused(lib.qw_mx_experts(one, 1, 64, one, 0, 64, 64, 4, 0, *weights, 0, one, one, 1 << 30, None), b"experts")
     need = lib.qw_mx_experts_workspace_bytes(4, 2, 64, 64)
-    assert lib.qw_mx_experts(one, 1, 4, 64, None, one, 2, 64, 64, 4, 0, one, one, one, one, one, one, 0, one, one,
-                             need - 1, None) == _lib.QW_ERR_WORKSPACE
+    assert lib.qw_mx_experts(one, 1, 64, one, 2, 64, 64, 4, 0, *weights, 0, one, one, need - 1,
+                             None) == _lib.QW_ERR_WORKSPACE
     need = lib.qw_mx_matmul_backward_workspace_bytes(4, 8, 64, 1)
     assert lib.qw_mx_matmul_backward(one, 1, 4, one, one, 8, 64, one, one, need - 1, None) == _lib.QW_ERR_WORKSPACE
     # nothing to do is no error
     assert lib.qw_mx_quantize(None, 0, 0, 64, 64, None, None, None) == _lib.QW_OK
-    assert route(None, 0, 64, 2, 0, None, 8, 1, 2, 1, 1.0, None, None, None, None, None) == _lib.QW_OK
+    assert route(None, 0, 64, 2, 0, None, 8, 1, 2, 1, 1.0, None, None, None, None) == _lib.QW_OK
 
 
 def test_oracle_rounds_to_the_nearest_value_with_ties_to_even():
