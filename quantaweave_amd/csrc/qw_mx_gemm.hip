@@ -130,7 +130,8 @@ __global__ __launch_bounds__(MX_THREADS) void mx_gemm_kernel(
   auto set_slots = [&] {
     auto addr = [](const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); };
     const int64_t w_row0 = static_cast<int64_t>(req.e) * n + req.n0;
-    const uint32_t x_end = req.count - 1, w_end = n - 1 - req.n0;
+    // (the matrix's last row where the tile has it: bytes from the tile's first row, within 32 bits)
+    const uint32_t x_end = req.count - 1, w_end = min(n - 1 - req.n0, MX_NB - 1);
 #pragma unroll
     for (int q = 0; q < CL; ++q) {
       const int g = code_group(q), gw = g - AG;

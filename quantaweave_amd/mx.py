@@ -21,6 +21,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _hip, _lib
 
@@ -135,6 +136,7 @@ class _MxMatmul(torch.autograd.Function):
         return _matmul(rows, stride, codes, scales)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad: Tensor):
         if not ctx.needs_input_grad[0]:
             return None, None, None

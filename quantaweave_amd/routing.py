@@ -14,6 +14,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _hip, _lib
 
@@ -53,6 +54,7 @@ class _RouteExperts(torch.autograd.Function):
         return index, weight, scores
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, _index, d_weight, d_scores):
         scores, index = ctx.saved_tensors
         top_k, score, _bias, _groups, _top_groups, _group_score, renormalize, scale = ctx.rule

@@ -123,6 +123,30 @@ def test_matmul_leading_dims_strides_and_alignment():
             close(got.reshape(-1, 48), want, ref.allowed(want, err, torch.bfloat16))
 
 
+@pytest.mark.parametrize("rows", [3, 17])  # both kernels
+def test_matmul_of_a_matrix_past_32_bit_offsets(rows):
+    n, k = (1 << 20) + 300, 8192  # 4.3 GB of codes
+    x = ref.rows(gen(17), rows, k, torch.bfloat16)
+    on_gpu = torch.Generator("cuda").manual_seed(17)
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=on_gpu)
+    scales = torch.randint(120, 132, (n, k // 32), dtype=torch.uint8, device="cuda", generator=on_gpu)
+    got = qa.mx_matmul(x.cuda(), codes, scales)
+    for at in (0, 256, n // 2 + 5, (1 << 20) - 30, n - 60):
+        part = slice(at, at + 60)
+        want, err = ref.matmul(x, codes[part].cpu(), scales[part].cpu())
+        close(got[:, part], want, ref.allowed(want, err, torch.bfloat16))
+
+
+def test_a_second_derivative_is_refused():
+    g = gen(19)
+    x, w = torch.randn(4, 96, generator=g).cuda().requires_grad_(True), cuda(ref.stored(g, 8, 96))
+    z = torch.randn(4, 16, generator=g).cuda().requires_grad_(True)
+    for y, leaf in ((qa.mx_matmul(x, *w), x), (qa.route_experts(z, 2)[1], z)):
+        (first,) = torch.autograd.grad(y.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
+
+
 def test_matmul_nan_and_infinite_rows_stay_in_their_rows():
     g = gen(5)
     for rows in (5, 80):
