@@ -452,8 +452,9 @@ int launch_sel(const MxProduct& p, hipStream_t stream) {
 
 }  // namespace
 
-// Dense rows: the chunk height whose tiles cost the fewest rounds of the chip (a
-// tile costs its rows and the loads of its weight rows).
+// Dense rows: the chunk height whose tiles cost the fewest rounds of the chip.  A
+// tile costs its rows and, as about 96 rows more, its start and its weight rows (a
+// slice of 320 rows about 2000 cycles, the start and store of a tile as much as five).
 int mx_dense_chunk(int64_t rows, int64_t n) {
   int best = 64;
   int64_t cost = INT64_MAX;
