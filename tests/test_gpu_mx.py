@@ -96,7 +96,8 @@ def test_dequantise_rounds_once(dtype):
 
 
 SHAPES = [(1, 64, 7), (1, 2048, 7168), (3, 200, 33), (16, 1408, 64), (17, 128, 130), (40, 33, 16), (64, 512, 256),
-          (65, 1000, 301), (130, 640, 96), (200, 2048, 512), (333, 384, 1000), (1, 1, 1), (700, 256, 260)]
+          (65, 1000, 301), (130, 640, 96), (200, 2048, 512), (333, 384, 1000), (1, 1, 1), (700, 256, 260),
+          (2, 4500, 40), (16, 9000, 33), (20, 5000, 70)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -219,7 +220,8 @@ def grouped(g, counts, d, f, dtype, tail=0):
 
 
 GROUPS = [([1], 64, 128), ([0, 5, 37, 1, 0, 64, 33, 2], 128, 96), ([3, 0, 17], 200, 264), ([16, 15, 1], 256, 33),
-          ([0, 0, 0], 64, 64), ([90, 300, 0, 21], 384, 320), ([2] * 40, 512, 128), ([129, 1], 1000, 200)]
+          ([0, 0, 0], 64, 64), ([90, 300, 0, 21], 384, 320), ([2] * 40, 512, 128), ([129, 1], 1000, 200),
+          ([0, 70, 0, 1, 0, 0, 3], 256, 128), ([3, 1], 2300, 160), ([2, 5], 264, 2400)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
