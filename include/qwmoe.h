@@ -526,7 +526,8 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
                  size_t workspace_bytes, void* stream);
 
 /* grad_x [rows, in_features] = grad_out [rows, out_features] @ W, the stored
- * matrix rounded to dtype first (exact for bf16 and fp32): the gradient of
+ * matrix exact but for entries of 2^128 and more (scale bytes 253 and 254), which
+ * are infinite, products summed in fp32 and rounded once: the gradient of
  * qw_mx_matmul with the quantisation of x passed over. */
 size_t qw_mx_matmul_backward_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features, int dtype);
 int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const void* codes, const void* scales,

@@ -48,7 +48,7 @@ struct TrArgs {
   void *c0, *c1;
   const int32_t* offsets;
   int64_t b_stride, c_stride;  // elements per expert
-  int lda, ldb, ldc;
+  int lda, ldb, ldc;  // B's rows hold ldb columns (a multiple of 8), of which n are columns of the result
   int rows, m, n, k, experts, parts;  // m: rows of an output matrix (red); k: reduction per part (rows)
 };
 
@@ -67,7 +67,8 @@ __device__ __forceinline__ s16x4 tr_read(const lds_s16x4* __restrict__ at) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>(at));
 }
 
-template <int DT, int SM, bool RED, bool BT, bool C32>
+// CDT: the result's type (DT, QW_F32, or QW_F16 of bf16 operands)
+template <int DT, int SM, bool RED, bool BT, int CDT>
 __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
   constexpr int TM = 32 * SM, NP = SM / 2, NT = 4;
   constexpr int A_STAGE = TM * TR_K * 2, B_STAGE = TR_N * TR_K * 2;
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
 #pragma unroll
   for (int q = 0; q < BL; ++q) {
     const int r = B_RPG * (wave + q * TR_WAVES) + lane / B_LPR, piece = lane % B_LPR;
-    const int c = min(n0 + 8 * (piece ^ (tr_swz(r) << 1)), p.n - 8);
+    const int c = min(n0 + 8 * (piece ^ (tr_swz(r) << 1)), p.ldb - 8);
     if constexpr (BT)  // 8 x 64 tiles of 1 KiB, 16-byte pieces XORed by the row
       b_off[q] = 2u * ((static_cast<uint32_t>(r / 8) * (p.n / 64) + c / 64) * 512u + (r % 8) * 64 +
                        8 * ((c / 8 % 8) ^ ((r >> 1) & 7)));
@@ -262,7 +263,9 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
 
   // ---- lane holds row l16 of sub-tile (wm + 2 i), columns 4 lq .. 4 lq + 3 of each 16-column tile ----
   const int64_t c_row0 = RED ? m0 : row0;
-  char* const c = static_cast<char*>(which ? p.c1 : p.c0) + (RED ? e * p.c_stride : 0) * (C32 ? 4 : 2);
+  char* const c = static_cast<char*>(which ? p.c1 : p.c0) + (RED ? e * p.c_stride : 0) * (CDT == QW_F32 ? 4 : 2);
+  // four columns go as one store where every row of the result starts on as many
+  const bool fours = CDT == QW_F32 || (p.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(c) % 8 == 0);
 #pragma unroll
   for (int i = 0; i < SM; ++i) {
     const int m = (wm + 2 * i) * 16 + l16;
@@ -273,21 +276,26 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
       const int n = wn * 64 + 16 * t + 4 * lq;
       if (n0 + n >= p.n) continue;
       const f32x4 v = acc[i][t];
-      if constexpr (C32)
+      if constexpr (CDT == QW_F32) {
         *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(c) + row + n) = v;
-      else
+      } else if (fours) {
         *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(c) + row + n) =
-            make_uint2(pack_half2<DT>(v[0], v[1]), pack_half2<DT>(v[2], v[3]));
+            make_uint2(pack_half2<CDT>(v[0], v[1]), pack_half2<CDT>(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (n0 + n + u < p.n) reinterpret_cast<uint16_t*>(c)[row + n + u] = f32_to_half<CDT>(v[u]);
+      }
     }
   }
 }
 
-template <int DT, int SM, bool RED, bool BT, bool C32>
+template <int DT, int SM, bool RED, bool BT, int CDT>
 int launch_tr(const TrArgs& a, int64_t blocks, hipStream_t stream) {
   constexpr int lds = tr_stages<SM>() * (32 * SM + TR_N) * TR_K * 2;
-  const hipError_t attr = reserve_lds<gemm_tr_kernel<DT, SM, RED, BT, C32>>(lds);
+  const hipError_t attr = reserve_lds<gemm_tr_kernel<DT, SM, RED, BT, CDT>>(lds);
   if (attr != hipSuccess) return set_error(QW_ERR_HIP, "cannot reserve LDS: %s", hipGetErrorString(attr));
-  gemm_tr_kernel<DT, SM, RED, BT, C32><<<static_cast<unsigned>(blocks), TR_THREADS, lds, stream>>>(a);
+  gemm_tr_kernel<DT, SM, RED, BT, CDT><<<static_cast<unsigned>(blocks), TR_THREADS, lds, stream>>>(a);
   QW_LAUNCH_CHECK("gemm_tr_kernel");
   return QW_OK;
 }
@@ -324,8 +332,11 @@ bool gemm_tr_dx_fits(const void* gy, const void* w, const void* gx, int64_t E, i
          aligned(gx);
 }
 
+// w_pitch: elements of a row of w, K or more, a multiple of 8.  gx_dtype: dtype, or
+// QW_F16 with plain bf16 operands; such a gx may have any K and start anywhere.
 int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1, int dtype, bool tiled, int64_t E,
-               int64_t N, int64_t K, const int32_t* offsets, int64_t rows, void* gx, hipStream_t stream) {
+               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx, int gx_dtype,
+               hipStream_t stream) {
   TrArgs a{};
   a.a0 = static_cast<const uint16_t*>(gy0);
   a.a1 = static_cast<const uint16_t*>(gy1 ? gy1 : gy0);
@@ -333,9 +344,10 @@ int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1,
   a.b1 = static_cast<const uint16_t*>(w1 ? w1 : w0);
   a.c0 = a.c1 = gx;
   a.offsets = offsets;
-  a.b_stride = N * K;
+  a.b_stride = N * w_pitch;
   a.lda = static_cast<int>(N);
-  a.ldb = a.ldc = a.n = static_cast<int>(K);
+  a.ldb = static_cast<int>(w_pitch);
+  a.ldc = a.n = static_cast<int>(K);
   a.rows = static_cast<int>(rows);
   a.k = static_cast<int>(N);
   a.experts = static_cast<int>(E);
@@ -343,14 +355,17 @@ int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1,
   const int64_t nt = ceil_div(K, TR_N);
   const bool tall = tall_tiles(row_tiles(rows, E, 256) * nt);
   const int64_t blocks = kXcds * nt * ceil_div(ceil_div(rows, tall ? 256 : 128) + E, kXcds);
-  auto go = [&](auto dt, auto bt) {
-    return tall ? launch_tr<decltype(dt)::value, 8, false, decltype(bt)::value, false>(a, blocks, stream)
-                : launch_tr<decltype(dt)::value, 4, false, decltype(bt)::value, false>(a, blocks, stream);
+  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many tiles for one product");
+  auto go = [&](auto dt, auto bt, auto cdt) {
+    constexpr int DT = decltype(dt)::value, CDT = decltype(cdt)::value;
+    return tall ? launch_tr<DT, 8, false, decltype(bt)::value, CDT>(a, blocks, stream)
+                : launch_tr<DT, 4, false, decltype(bt)::value, CDT>(a, blocks, stream);
   };
   using H = std::integral_constant<int, QW_F16>;
   using B = std::integral_constant<int, QW_BF16>;
-  if (dtype == QW_F16) return tiled ? go(H{}, std::true_type{}) : go(H{}, std::false_type{});
-  return tiled ? go(B{}, std::true_type{}) : go(B{}, std::false_type{});
+  if (gx_dtype != dtype) return go(B{}, std::false_type{}, H{});
+  if (dtype == QW_F16) return tiled ? go(H{}, std::true_type{}, H{}) : go(H{}, std::false_type{}, H{});
+  return tiled ? go(B{}, std::true_type{}, B{}) : go(B{}, std::false_type{}, B{});
 }
 
 // dW of one product, or of two with the same x (gy1, gw1 non-null).
@@ -377,14 +392,16 @@ int gemm_tr_dw(const void* gy0, const void* gy1, const void* x, int dtype, int64
   const int64_t nt = ceil_div(K, TR_N), per = a.parts * E;
   const bool tall = tall_tiles(static_cast<double>(per * nt * ceil_div(N, 256)));
   const int64_t blocks = kXcds * per * ceil_div(nt * ceil_div(N, tall ? 256 : 128), kXcds);
-  auto go = [&](auto dt, auto c32) {
-    return tall ? launch_tr<decltype(dt)::value, 8, true, false, decltype(c32)::value>(a, blocks, stream)
-                : launch_tr<decltype(dt)::value, 4, true, false, decltype(c32)::value>(a, blocks, stream);
+  auto go = [&](auto dt, auto cdt) {
+    constexpr int DT = decltype(dt)::value, CDT = decltype(cdt)::value;
+    return tall ? launch_tr<DT, 8, true, false, CDT>(a, blocks, stream)
+                : launch_tr<DT, 4, true, false, CDT>(a, blocks, stream);
   };
   using H = std::integral_constant<int, QW_F16>;
   using B = std::integral_constant<int, QW_BF16>;
-  if (dtype == QW_F16) return gw_f32 ? go(H{}, std::true_type{}) : go(H{}, std::false_type{});
-  return gw_f32 ? go(B{}, std::true_type{}) : go(B{}, std::false_type{});
+  using F = std::integral_constant<int, QW_F32>;
+  if (dtype == QW_F16) return gw_f32 ? go(H{}, F{}) : go(H{}, H{});
+  return gw_f32 ? go(B{}, F{}) : go(B{}, B{});
 }
 
 }  // namespace qw

@@ -8,6 +8,9 @@ int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dt
                             int64_t K, const int32_t* offsets, int64_t rows, int64_t max_rows_per_expert, void* gx,
                             int accumulate, void* gw, int gw_dtype, void* ws, size_t ws_bytes, hipStream_t stream);
 size_t grouped_backward_workspace_bytes(int64_t E, int64_t N, int64_t K, int64_t rows, int dtype);
+int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1, int dtype, bool tiled, int64_t E,
+               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx, int gx_dtype,
+               hipStream_t stream);
 
 namespace {
 
@@ -36,6 +39,27 @@ int check_matrix(const void* codes, const void* scales, const char* what) {
 MxMatrix matrix(const void* codes, const void* scales) {
   return MxMatrix{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales)};
 }
+
+// The gradient of fp16 rows.  Stored weights reach from 2^-128 to 6 * 2^127, past
+// fp16 at both ends, so the matrix is held in bf16, which has their range and more
+// bits than a code; fp16's eleven bits of grad_out go as two bf16 numbers, whose
+// products with it are summed in one fp32 accumulator.  (The matrix in fp16 took
+// half the instructions and was right for scales of 2^-23 to 2^13 alone.)
+struct HalfGradient {
+  int64_t n, pitch;  // the reduction and the matrix's rows, padded to what the tiles take
+  int32_t* offsets;
+  uint16_t *w, *high, *low;
+  size_t bytes;
+  HalfGradient(void* workspace, int64_t rows, int64_t out_features, int64_t in_features)
+      : n(ceil_div(out_features, 64) * 64), pitch(ceil_div(in_features, 8) * 8) {
+    Carver c(workspace);
+    offsets = c.take<int32_t>(2);
+    w = c.take<uint16_t>(static_cast<size_t>(n) * pitch);
+    high = c.take<uint16_t>(static_cast<size_t>(rows) * n);
+    low = c.take<uint16_t>(static_cast<size_t>(rows) * n);
+    bytes = c.used + 256;
+  }
+};
 
 __global__ void mx_offsets_kernel(int32_t* offsets, int rows) {
   offsets[0] = 0;
@@ -76,7 +100,7 @@ int qw_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_
   QW_REQUIRE(out != nullptr, "out is required");
   st = check_matrix(codes, scales, "input");
   if (st) return st;
-  return mx_dequantize(codes, scales, rows, cols, out, out_dtype, as_stream(stream));
+  return mx_dequantize(codes, scales, rows, cols, out, out_dtype, rows, as_stream(stream));
 }
 
 size_t qw_mx_matmul_workspace_bytes(const void* x, int act_dtype, int64_t x_row_stride, int64_t rows,
@@ -130,6 +154,7 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
 
 size_t qw_mx_matmul_backward_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features, int dtype) {
   if (rows < 1 || out_features < 1 || in_features < 1) return 0;
+  if (dtype == QW_F16) return HalfGradient(nullptr, rows, out_features, in_features).bytes;
   Carver c(nullptr);
   c.take<int32_t>(2);
   c.take<char>(static_cast<size_t>(out_features) * in_features * (dtype == QW_F32 ? 4 : 2));
@@ -153,6 +178,16 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(QW_ERR_WORKSPACE, "mx_matmul_backward needs a workspace of %zu bytes, got %zu", need,
                      workspace_bytes);
+  if (dtype == QW_F16) {
+    const HalfGradient g(workspace, rows, out_features, in_features);
+    QW_REQUIRE(g.n <= 1 << 22, "out_features out of range for a gradient: %lld", (long long)out_features);
+    mx_offsets_kernel<<<1, 1, 0, as_stream(stream)>>>(g.offsets, static_cast<int>(rows));
+    QW_LAUNCH_CHECK("mx_offsets_kernel");
+    st = mx_dequantize(codes, scales, out_features, g.pitch, g.w, QW_BF16, g.n, as_stream(stream));
+    if (!st) st = mx_split(grad_out, rows, out_features, g.n, g.high, g.low, as_stream(stream));
+    return st ? st : gemm_tr_dx(g.high, g.low, g.w, g.w, QW_BF16, false, 1, g.n, in_features, g.pitch, g.offsets, rows,
+                                grad_x, QW_F16, as_stream(stream));
+  }
   Carver c(workspace);
   int32_t* offsets = c.take<int32_t>(2);
   void* w = c.take<char>(static_cast<size_t>(out_features) * in_features * (dtype == QW_F32 ? 4 : 2));
@@ -160,7 +195,7 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
   void* ws = c.take<char>(inner);
   mx_offsets_kernel<<<1, 1, 0, as_stream(stream)>>>(offsets, static_cast<int>(rows));
   QW_LAUNCH_CHECK("mx_offsets_kernel");
-  st = mx_dequantize(codes, scales, out_features, in_features, w, dtype, as_stream(stream));
+  st = mx_dequantize(codes, scales, out_features, in_features, w, dtype, out_features, as_stream(stream));
   if (st) return st;
   return grouped_matmul_backward(grad_out, nullptr, w, dtype, dtype, 1, out_features, in_features, offsets, rows, rows,
                                  grad_x, 0, nullptr, dtype, ws, inner, as_stream(stream));

@@ -69,7 +69,11 @@ int mx_prepare(const void* x, int dtype, int64_t rows, int64_t cols, int64_t str
 
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, void* codes, void* scales,
                 hipStream_t stream);
+// The first `cols` columns (the stored padding may be among them) of each row; rows
+// behind the stored ones up to out_rows become zeros.
 int mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
-                  hipStream_t stream);
+                  int64_t out_rows, hipStream_t stream);
+// Rows of fp16 numbers as sums of two bf16 rows, padded with zeros to `pitch` columns.
+int mx_split(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* high, void* low, hipStream_t stream);
 
 }  // namespace qw

@@ -159,7 +159,9 @@ def mx_matmul(x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
     """x [..., in] times a stored matrix [out, in], transposed: [..., out] of x's type.
 
     x (float32, bfloat16 or float16) is quantised on the way; the sum is fp32,
-    rounded once.  Differentiable in x (the stored matrix takes no gradient)."""
+    rounded once.  Differentiable in x (the stored matrix takes no gradient):
+    grad_x = grad_out @ W, summed in fp32 and rounded once, with stored values
+    of 2^128 and more (scales 253 and 254) infinite."""
     dev = _device(x, "mx_matmul")
     _hip.act_code(x, "mx_matmul")
     if x.dim() < 1 or x.size(-1) < 1:

@@ -187,6 +187,32 @@ def test_matmul_gradient(dtype, rows, cols, n):
     assert torch.equal(y.detach(), qa.mx_matmul(x.cuda(), *cuda(w)))
 
 
+@pytest.mark.parametrize("rows,cols,n", [(1, 33, 7), (5, 96, 64), (70, 264, 130), (300, 512, 200)])
+@pytest.mark.parametrize("low,high", [(87, 158), (90, 91), (100, 101), (141, 142), (150, 151), (60, 230)])
+def test_fp16_gradient_over_the_range_of_the_scales(rows, cols, n, low, high):
+    """Stored weights past fp16 at either end: what fp16 can hold of the result is right, the rest is infinite or 0."""
+    g = gen(rows + cols + low)
+    w = ref.stored(g, n, cols, low=low, high=high)
+    # a block of columns has the scales of its first row give or take two, so that the results have every size
+    w = (w[0], (w[1][:1].int() + torch.randint(-2, 3, w[1].shape, generator=g)).clamp(0, 254).to(torch.uint8))
+    dy = torch.randn(rows, n, generator=g) * torch.exp2(torch.randint(-14, 8, (rows, 1), generator=g))
+    dy[torch.rand(rows, n, generator=g) < 0.3] = 0.0
+    dy[0] = 0.0
+    dy = dy.half()
+    x = ref.rows(g, rows, cols, torch.float16).cuda().requires_grad_(True)
+    (gx,) = torch.autograd.grad(qa.mx_matmul(x, *cuda(w)), x, dy.cuda())
+    gx = gx.cpu().double()
+    assert not gx[0].any() and not torch.isnan(gx).any()
+    wv = ref.values(*w, cols)
+    want = dy.double() @ wv
+    # dy as two numbers whose magnitudes add up to at most 1 + 2^-7 of it: 2 n products, each exact, and their sums
+    err = (2 * n + 8) * ref.EPS24 * (1 + 2.0 ** -7) * (dy.double().abs() @ wv.abs())
+    beyond = want.abs() + err >= 65520.0  # rounds to an infinity, or may
+    assert torch.isinf(gx[want.abs() - err >= 65520.0]).all()
+    bad = ~beyond & ~((gx - want).abs() <= ref.allowed(want, err, torch.float16))
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}"
+
+
 def test_matmul_gradient_is_a_difference_of_the_product_on_the_grid():
     """Where x moves from grid value to grid value the product's difference is the gradient times it."""
     g = gen(21)
