@@ -509,6 +509,15 @@ int gemm_grouped_forward(const void* x, const void* w, int dtype, int64_t E, int
                                                 stream);
 }
 
+// gx = gy . w of one group, bf16, w [N, w_pitch] with K columns: N % 64 == 0, K % 4 == 0,
+// operands and gx on 16 bytes.
+int gemm_dx(const void* gy, const void* w, int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows,
+            void* gx, hipStream_t stream) {
+  return launch_gemm<QW_BF16, MODE_ROWS, false, true>(gy, N, w, w_pitch, N * w_pitch, gx, K, 0, offsets,
+                                                      static_cast<int>(rows), 0, static_cast<int>(K),
+                                                      static_cast<int>(N), 1, rows, stream);
+}
+
 // Backward of gemm_grouped_forward on the matrix cores (bf16 or fp16, DT):
 //   gx = gy . w[e] (+ gx when accumulate), gw[e] = gy_e^T . x_e (fp32 when gw_f32).
 template <int DT>

@@ -332,8 +332,8 @@ bool gemm_tr_dx_fits(const void* gy, const void* w, const void* gx, int64_t E, i
          aligned(gx);
 }
 
-// w_pitch: elements of a row of w, K or more, a multiple of 8.  gx_dtype: dtype, or
-// QW_F16 with plain bf16 operands; such a gx may have any K and start anywhere.
+// w_pitch: elements of a row of w, K or more, a multiple of 8; with it K may be any
+// and gx start anywhere.  gx_dtype: dtype, or QW_F16 with plain bf16 operands.
 int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1, int dtype, bool tiled, int64_t E,
                int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx, int gx_dtype,
                hipStream_t stream) {

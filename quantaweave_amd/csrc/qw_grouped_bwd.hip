@@ -151,10 +151,11 @@ __device__ const uint4 g_fb_zero = {0u, 0u, 0u, 0u};  // pieces past the end of 
 // RED: grad_W_e[n, k] = sum over the rows r of expert e of gy[r, n] a[r, k], a = x
 //      (exactly zero without rows); block (k tile, n tile, expert).
 // else: grad_x[r, k] (+)= sum_n gy[r, n] a[n, k], a = W_e; block (k tile, row tile, expert).
+// Rows of a hold K columns (K % 4 == 0), rows of the result the first `cols` of them.
 template <bool RED>
 __global__ __launch_bounds__(256) void grouped_f32_kernel(const float* __restrict__ gy, const float* __restrict__ a,
-                                                          const int32_t* __restrict__ offsets, int N, int K, int rows,
-                                                          int accumulate, float* __restrict__ out) {
+                                                          const int32_t* __restrict__ offsets, int N, int K, int cols,
+                                                          int rows, int accumulate, float* __restrict__ out) {
   __shared__ __attribute__((aligned(1024))) float ring[FB_ST][2][FB_OPER];
   const int e = blockIdx.z;
   const int lo = min(max(offsets[e], 0), rows), hi = min(offsets[e + 1], rows);
@@ -247,7 +248,8 @@ __global__ __launch_bounds__(256) void grouped_f32_kernel(const float* __restric
     }
   }
   // lane holds row wm*32 + 16i + l16, columns wn*32 + 16t + 4lq .. +3
-  float* const base = out + (RED ? static_cast<int64_t>(e) * N + m0 : static_cast<int64_t>(lo) + m0) * K;
+  float* const base = out + (RED ? static_cast<int64_t>(e) * N + m0 : static_cast<int64_t>(lo) + m0) * cols;
+  const bool fours = cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int m = wm * 32 + 16 * i + l16;
@@ -255,9 +257,16 @@ __global__ __launch_bounds__(256) void grouped_f32_kernel(const float* __restric
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int k = k0 + wn * 32 + 16 * t + 4 * lq;
-      if (k >= K) continue;  // K % 4 == 0: wholly inside or past the end
-      bf32x4* o = reinterpret_cast<bf32x4*>(base + static_cast<int64_t>(m) * K + k);
+      if (k >= cols) continue;
+      float* const at = base + static_cast<int64_t>(m) * cols + k;
+      bf32x4* o = reinterpret_cast<bf32x4*>(at);
       bf32x4 v = acc[i][t];
+      if (!fours) {  // (never with accumulate)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k + j < cols) at[j] = v[j];
+        continue;
+      }
       if (!RED && accumulate) {
         const bf32x4 old = *o;
 #pragma unroll
@@ -342,7 +351,7 @@ int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dt
     const dim3 g(static_cast<unsigned>(ceil_div(K, FB_T)), static_cast<unsigned>(ceil_div(per, FB_T)),
                  static_cast<unsigned>(E));
     grouped_f32_kernel<false><<<g, 256, 0, stream>>>(static_cast<const float*>(gy), static_cast<const float*>(w),
-                                                     offsets, n, k, r, accumulate, static_cast<float*>(gx));
+                                                     offsets, n, k, k, r, accumulate, static_cast<float*>(gx));
     QW_LAUNCH_CHECK("grouped_f32_kernel");
     gx = nullptr;
   }
@@ -350,7 +359,7 @@ int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dt
     const dim3 g(static_cast<unsigned>(ceil_div(K, FB_T)), static_cast<unsigned>(ceil_div(N, FB_T)),
                  static_cast<unsigned>(E));
     grouped_f32_kernel<true><<<g, 256, 0, stream>>>(static_cast<const float*>(gy), static_cast<const float*>(x),
-                                                    offsets, n, k, r, 0, static_cast<float*>(gw));
+                                                    offsets, n, k, k, r, 0, static_cast<float*>(gw));
     QW_LAUNCH_CHECK("grouped_f32_kernel");
     gw = nullptr;
   }
@@ -373,6 +382,17 @@ int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dt
     else grouped_dw_kernel<QW_BF16, QW_BF16><<<g, 256, 0, stream>>>(gy, x, offsets, n, k, r, gw);
     QW_LAUNCH_CHECK("grouped_dw_kernel");
   }
+  return QW_OK;
+}
+
+// gx = gy . w of one group, fp32, w [N, w_pitch] with K columns: N and w_pitch multiples
+// of 4, gy and w on 16 bytes.
+int grouped_f32_dx(const float* gy, const float* w, int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets,
+                   int64_t rows, float* gx, hipStream_t stream) {
+  const dim3 g(static_cast<unsigned>(ceil_div(K, FB_T)), static_cast<unsigned>(ceil_div(rows, FB_T)));
+  grouped_f32_kernel<false><<<g, 256, 0, stream>>>(gy, w, offsets, static_cast<int>(N), static_cast<int>(w_pitch),
+                                                   static_cast<int>(K), static_cast<int>(rows), 0, gx);
+  QW_LAUNCH_CHECK("grouped_f32_kernel");
   return QW_OK;
 }
 

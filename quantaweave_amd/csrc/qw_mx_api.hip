@@ -7,7 +7,12 @@ namespace qw {
 int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dtype, int wfmt, int64_t E, int64_t N,
                             int64_t K, const int32_t* offsets, int64_t rows, int64_t max_rows_per_expert, void* gx,
                             int accumulate, void* gw, int gw_dtype, void* ws, size_t ws_bytes, hipStream_t stream);
-size_t grouped_backward_workspace_bytes(int64_t E, int64_t N, int64_t K, int64_t rows, int dtype);
+int grouped_f32_dx(const float* gy, const float* w, int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets,
+                   int64_t rows, float* gx, hipStream_t stream);
+int gemm_dx(const void* gy, const void* w, int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows,
+            void* gx, hipStream_t stream);
+bool gemm_tr_dx_fits(const void* gy, const void* w, const void* gx, int64_t E, int64_t N, int64_t K, int64_t rows,
+                     bool pair, bool tiles128);
 int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1, int dtype, bool tiled, int64_t E,
                int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx, int gx_dtype,
                hipStream_t stream);
@@ -40,23 +45,38 @@ MxMatrix matrix(const void* codes, const void* scales) {
   return MxMatrix{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales)};
 }
 
-// The gradient of fp16 rows.  Stored weights reach from 2^-128 to 6 * 2^127, past
-// fp16 at both ends, so the matrix is held in bf16, which has their range and more
-// bits than a code; fp16's eleven bits of grad_out go as two bf16 numbers, whose
-// products with it are summed in one fp32 accumulator.  (The matrix in fp16 took
-// half the instructions and was right for scales of 2^-23 to 2^13 alone.)
-struct HalfGradient {
-  int64_t n, pitch;  // the reduction and the matrix's rows, padded to what the tiles take
+// Workspace of the rows' gradient, gx = gy . W on the framework's backward products.
+//
+// Whatever the widths, the matrix cores take it: W is dequantised into a copy of its
+// own, so its rows are padded with zeros to the tiles' slices of the reduction (64
+// rows; 4 in fp32) and its columns to whole loads, and gy is copied to the padded
+// width where that differs (30 rows, 1000 columns, 3001 outputs, whole calls: bf16 448
+// us on the vector ALU, 75 so; fp32 with 64 rows and 1001 columns 527 and 87).
+//
+// The matrix is held in bf16 for 16-bit rows, fp16 ones too: stored weights reach
+// from 2^-128 to 6 * 2^127, past fp16 at both ends, and bf16 has their range and more
+// bits than a code.  fp16's eleven bits of gy then go as two bf16 numbers, whose
+// products with W are summed in one fp32 accumulator.  (The matrix in fp16 took half
+// the instructions, 110 us instead of 210 for 1024 rows, 1024 columns and 7168 outputs,
+// and was right for scales of 2^-23 to 2^13 alone.)
+struct RowsGradient {
+  int64_t n, pitch;  // W's padded rows and columns
+  bool copied;       // gy is taken from `rows`
   int32_t* offsets;
-  uint16_t *w, *high, *low;
+  void* w;
+  void* rows;        // gy, padded; fp16: its high parts
+  void* low;         // fp16: its low parts
   size_t bytes;
-  HalfGradient(void* workspace, int64_t rows, int64_t out_features, int64_t in_features)
-      : n(ceil_div(out_features, 64) * 64), pitch(ceil_div(in_features, 8) * 8) {
+  RowsGradient(void* workspace, int64_t count, int64_t out_features, int64_t in_features, int dtype) {
+    const int64_t slice = dtype == QW_F32 ? 4 : 64, load = dtype == QW_F32 ? 4 : 8, size = dtype == QW_F32 ? 4 : 2;
+    n = ceil_div(out_features, slice) * slice;
+    pitch = ceil_div(in_features, load) * load;
+    copied = dtype == QW_F16 || n != out_features;
     Carver c(workspace);
     offsets = c.take<int32_t>(2);
-    w = c.take<uint16_t>(static_cast<size_t>(n) * pitch);
-    high = c.take<uint16_t>(static_cast<size_t>(rows) * n);
-    low = c.take<uint16_t>(static_cast<size_t>(rows) * n);
+    w = c.take<char>(static_cast<size_t>(n) * pitch * size);
+    rows = c.take<char>(copied ? static_cast<size_t>(count) * n * size : 0);
+    low = c.take<char>(dtype == QW_F16 ? static_cast<size_t>(count) * n * size : 0);
     bytes = c.used + 256;
   }
 };
@@ -154,12 +174,7 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
 
 size_t qw_mx_matmul_backward_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features, int dtype) {
   if (rows < 1 || out_features < 1 || in_features < 1) return 0;
-  if (dtype == QW_F16) return HalfGradient(nullptr, rows, out_features, in_features).bytes;
-  Carver c(nullptr);
-  c.take<int32_t>(2);
-  c.take<char>(static_cast<size_t>(out_features) * in_features * (dtype == QW_F32 ? 4 : 2));
-  c.take<char>(grouped_backward_workspace_bytes(1, out_features, in_features, rows, dtype));
-  return c.used + 256;
+  return RowsGradient(nullptr, rows, out_features, in_features, dtype).bytes;
 }
 
 int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const void* codes, const void* scales,
@@ -178,27 +193,34 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(QW_ERR_WORKSPACE, "mx_matmul_backward needs a workspace of %zu bytes, got %zu", need,
                      workspace_bytes);
-  if (dtype == QW_F16) {
-    const HalfGradient g(workspace, rows, out_features, in_features);
-    QW_REQUIRE(g.n <= 1 << 22, "out_features out of range for a gradient: %lld", (long long)out_features);
-    mx_offsets_kernel<<<1, 1, 0, as_stream(stream)>>>(g.offsets, static_cast<int>(rows));
-    QW_LAUNCH_CHECK("mx_offsets_kernel");
-    st = mx_dequantize(codes, scales, out_features, g.pitch, g.w, QW_BF16, g.n, as_stream(stream));
-    if (!st) st = mx_split(grad_out, rows, out_features, g.n, g.high, g.low, as_stream(stream));
-    return st ? st : gemm_tr_dx(g.high, g.low, g.w, g.w, QW_BF16, false, 1, g.n, in_features, g.pitch, g.offsets, rows,
-                                grad_x, QW_F16, as_stream(stream));
-  }
-  Carver c(workspace);
-  int32_t* offsets = c.take<int32_t>(2);
-  void* w = c.take<char>(static_cast<size_t>(out_features) * in_features * (dtype == QW_F32 ? 4 : 2));
-  const size_t inner = grouped_backward_workspace_bytes(1, out_features, in_features, rows, dtype);
-  void* ws = c.take<char>(inner);
-  mx_offsets_kernel<<<1, 1, 0, as_stream(stream)>>>(offsets, static_cast<int>(rows));
+  const RowsGradient g(workspace, rows, out_features, in_features, dtype);
+  QW_REQUIRE(ceil_div(rows, 64) <= 65535 && g.n <= 1 << 22, "sizes out of range for a gradient: %lld rows, %lld out_features",
+             (long long)rows, (long long)out_features);
+  const hipStream_t s = as_stream(stream);
+  mx_offsets_kernel<<<1, 1, 0, s>>>(g.offsets, static_cast<int>(rows));
   QW_LAUNCH_CHECK("mx_offsets_kernel");
-  st = mx_dequantize(codes, scales, out_features, in_features, w, dtype, out_features, as_stream(stream));
+  const int wdt = dtype == QW_F32 ? QW_F32 : QW_BF16;
+  auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  if (!g.copied && !aligned(grad_out)) {  // no copy and no 16-byte loads: the vector-ALU kernel
+    st = mx_dequantize(codes, scales, out_features, in_features, g.w, wdt, out_features, s);
+    return st ? st : grouped_matmul_backward(grad_out, nullptr, g.w, dtype, dtype, 1, out_features, in_features,
+                                             g.offsets, rows, rows, grad_x, 0, nullptr, dtype, nullptr, 0, s);
+  }
+  st = mx_dequantize(codes, scales, out_features, g.pitch, g.w, wdt, g.n, s);
   if (st) return st;
-  return grouped_matmul_backward(grad_out, nullptr, w, dtype, dtype, 1, out_features, in_features, offsets, rows, rows,
-                                 grad_x, 0, nullptr, dtype, ws, inner, as_stream(stream));
+  if (dtype == QW_F16) st = mx_split(grad_out, rows, out_features, g.n, g.rows, g.low, s);
+  else if (g.copied) st = mx_pad(grad_out, dtype == QW_F32 ? 4 : 2, rows, out_features, g.n, g.rows, s);
+  if (st) return st;
+  const void* const gy = g.copied ? g.rows : grad_out;
+  if (dtype == QW_F32)
+    return grouped_f32_dx(static_cast<const float*>(gy), static_cast<const float*>(g.w), g.n, in_features, g.pitch,
+                          g.offsets, rows, static_cast<float*>(grad_x), s);
+  // tiles of 128 x 128 as in the grouped backward, which need whole fours and 16-byte rows of results
+  const bool tiles128 = dtype == QW_BF16 && in_features % 4 == 0 && aligned(grad_x);
+  if (tiles128 && !gemm_tr_dx_fits(gy, g.w, grad_x, 1, g.n, in_features, rows, false, true))
+    return gemm_dx(gy, g.w, g.n, in_features, g.pitch, g.offsets, rows, grad_x, s);
+  return gemm_tr_dx(gy, dtype == QW_F16 ? g.low : nullptr, g.w, dtype == QW_F16 ? g.w : nullptr, QW_BF16, false, 1, g.n,
+                    in_features, g.pitch, g.offsets, rows, grad_x, dtype, s);
 }
 
 size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t d_model, int64_t d_ff) {

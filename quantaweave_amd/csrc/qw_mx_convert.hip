@@ -144,6 +144,27 @@ __global__ __launch_bounds__(kConvertThreads) void mx_dequantize_kernel(const ui
   }
 }
 
+// Rows padded with zeros to `pitch` columns, a multiple of 4, four of them per lane.
+template <typename T>
+__global__ __launch_bounds__(kConvertThreads) void mx_pad_kernel(const T* __restrict__ x, int cols, int pitch,
+                                                                 int64_t total, bool fours, T* __restrict__ out) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvertThreads + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / (pitch / 4);
+  const int col = static_cast<int>(i - row * (pitch / 4)) * 4;
+  const T* const at = x + row * cols + col;
+  T4 v = {0, 0, 0, 0};
+  if (fours && col < cols) {
+    v = *reinterpret_cast<const T4*>(at);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < cols) v[k] = at[k];
+  }
+  reinterpret_cast<T4*>(out)[i] = v;
+}
+
 // fp16 numbers as the sum of two bf16 ones: the number rounded to eight bits, and
 // the rest, which has three bits at most (0 beside an infinity or a NaN).  Rows are
 // padded with zeros to `pitch` columns (whole eights).
@@ -213,6 +234,21 @@ int mx_prepare(const void* x, int dtype, int64_t rows, int64_t cols, int64_t str
   else if (dtype == QW_F16) go(mx_prepare_kernel<QW_F16>);
   else go(mx_prepare_kernel<QW_BF16>);
   QW_LAUNCH_CHECK("mx_prepare_kernel");
+  return QW_OK;
+}
+
+int mx_pad(const void* x, int size, int64_t rows, int64_t cols, int64_t pitch, void* out, hipStream_t stream) {
+  const int64_t total = rows * (pitch / 4), blocks = ceil_div(total, kConvertThreads);
+  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many rows to pad in one call");
+  const bool fours = cols % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * size) == 0;
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    mx_pad_kernel<T><<<static_cast<unsigned>(blocks), kConvertThreads, 0, stream>>>(
+        static_cast<const T*>(x), static_cast<int>(cols), static_cast<int>(pitch), total, fours, static_cast<T*>(out));
+  };
+  if (size == 4) go(uint32_t{0});
+  else go(uint16_t{0});
+  QW_LAUNCH_CHECK("mx_pad_kernel");
   return QW_OK;
 }
 

@@ -73,6 +73,8 @@ int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t st
 // behind the stored ones up to out_rows become zeros.
 int mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
                   int64_t out_rows, hipStream_t stream);
+// Rows padded with zeros to `pitch` columns (both in elements of `size` bytes, 2 or 4).
+int mx_pad(const void* x, int size, int64_t rows, int64_t cols, int64_t pitch, void* out, hipStream_t stream);
 // Rows of fp16 numbers as sums of two bf16 rows, padded with zeros to `pitch` columns.
 int mx_split(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* high, void* low, hipStream_t stream);
 

@@ -142,6 +142,8 @@ class _MxMatmul(torch.autograd.Function):
             return None, None, None
         codes, scales = ctx.saved_tensors
         grad = grad.to(ctx.dtype).contiguous()
+        if grad.data_ptr() % 16:
+            grad = grad.clone()  # the matrix cores' loads
         rows, n, k = grad.size(0), codes.size(0), ctx.cols
         gx = torch.empty(rows, k, dtype=ctx.dtype, device=grad.device)
         if rows and n:

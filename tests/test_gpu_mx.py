@@ -187,6 +187,37 @@ def test_matmul_gradient(dtype, rows, cols, n):
     assert torch.equal(y.detach(), qa.mx_matmul(x.cuda(), *cuda(w)))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,n", [(64, 1000, 3001), (1, 1000, 301), (700, 1000, 97), (2000, 333, 65),
+                                         (130, 12, 100), (33, 4, 7), (257, 1001, 192), (300, 6, 64), (40, 1, 1),
+                                         (5, 100, 128), (1200, 2052, 130)])
+def test_matmul_gradient_of_any_width(dtype, rows, cols, n):
+    """Widths that are no whole slices or loads of the matrix cores; a grad_out off 16 bytes; through the C entry
+    point a grad_out and a grad_x off 16 bytes, rows behind grad_x left as they were."""
+    g = gen(rows + cols * n)
+    w = ref.stored(g, n, cols)
+    dy = torch.randn(rows, n, generator=g).to(dtype)
+    wv = ref.values(*w, cols)
+    want = dy.double() @ wv
+    # fp32 sums of n exact products, of 2 n with fp16's two parts; fp32's own products are rounded
+    terms = {torch.float32: 2 * n + 8, torch.bfloat16: n + 8, torch.float16: (2 * n + 8) * (1 + 2.0 ** -7)}[dtype]
+    err = ref.allowed(want, terms * ref.EPS24 * (dy.double().abs() @ wv.abs()), dtype)
+    x = ref.rows(g, rows, cols, dtype).cuda().requires_grad_(True)
+    y = qa.mx_matmul(x, *cuda(w))
+    off = torch.empty(rows * n + 1, dtype=dtype, device="cuda")[1:].view(rows, n).copy_(dy)
+    for grad in (dy.cuda(), off):
+        close(torch.autograd.grad(y, x, grad, retain_graph=True)[0], want, err)
+    act, (codes, scales), lib = _hip.act_code(dy, "test"), cuda(w), _lib.load()
+    nbytes = lib.qw_mx_matmul_backward_workspace_bytes(rows, n, cols, act)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    for grad, start in ((dy.cuda(), 1), (off, 0)):
+        out = torch.full((start + rows * cols + 64,), 3.0, dtype=dtype, device="cuda")
+        _lib.call("qw_mx_matmul_backward", _hip.ptr(grad), act, rows, _hip.ptr(codes), _hip.ptr(scales), n, cols,
+                  _hip.ptr(out[start:]), _hip.ptr(ws), nbytes, _hip.stream(out.device))
+        close(out[start:start + rows * cols].view(rows, cols), want, err)
+        assert (out[:start] == 3.0).all() and (out[start + rows * cols:] == 3.0).all()
+
+
 @pytest.mark.parametrize("rows,cols,n", [(1, 33, 7), (5, 96, 64), (70, 264, 130), (300, 512, 200)])
 @pytest.mark.parametrize("low,high", [(87, 158), (90, 91), (100, 101), (141, 142), (150, 151), (60, 230)])
 def test_fp16_gradient_over_the_range_of_the_scales(rows, cols, n, low, high):

@@ -69,6 +69,15 @@ def test_entry_points_check_their_arguments_before_any_launch():
     assert route(None, 0, 64, 2, 0, None, 8, 1, 2, 1, 1.0, None, None, None, None) == _lib.QW_OK
 
 
+@pytest.mark.parametrize("dtype,size", [(_lib.QW_F32, 4), (_lib.QW_BF16, 2)])
+def test_the_gradient_of_rows_alone_takes_no_room_for_that_of_the_matrix(dtype, size):
+    """The matrix as numbers, and grad_out where its width is padded; no transposed copies of rows."""
+    need = _lib.load().qw_mx_matmul_backward_workspace_bytes
+    matrix = 7168 * 2048 * size
+    assert matrix <= need(8192, 7168, 2048, dtype) <= matrix + 1024
+    assert need(8192, 7001, 2048, dtype) <= matrix + 8192 * 7040 * size + 1024
+
+
 def test_oracle_rounds_to_the_nearest_value_with_ties_to_even():
     x = torch.tensor([[0.25, 0.26, 0.75, 0.74, 1.25, 1.75, 2.5, 3.5, 5.0, 5.01, 7.9, -0.25, -2.5, 4.0] + [0.0] * 18])
     want = [0, 0.5, 1, 0.5, 1, 2, 2, 4, 4, 6, 6, 0, -2, 4] + [0.0] * 18
