@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -57,6 +58,13 @@ def call_on(device: torch.device, name: str, *args) -> None:
     else:
         with torch.cuda.device(device):
             _lib.call(name, *args)
+
+
+def refuse_tangent(t: torch.Tensor, what: str) -> None:
+    """Called by an operator that hands `t` to its kernel without an autograd node:
+    a forward-mode tangent of t would be lost on the way."""
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not supported")
 
 
 _STREAM_KEY = "quantaweave stream"

@@ -163,11 +163,13 @@ def mx_matmul(x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
     x (float32, bfloat16 or float16) is quantised on the way; the sum is fp32,
     rounded once.  Differentiable in x (the stored matrix takes no gradient):
     grad_x = grad_out @ W, summed in fp32 and rounded once, with stored values
-    of 2^128 and more (scales 253 and 254) infinite."""
+    of 2^128 and more (scales 253 and 254) infinite.  Second and forward-mode
+    derivatives are refused."""
     dev = _device(x, "mx_matmul")
     _hip.act_code(x, "mx_matmul")
     if x.dim() < 1 or x.size(-1) < 1:
         raise ValueError(f"mx_matmul: rows of at least one column are needed, got shape {tuple(x.shape)}")
+    _hip.refuse_tangent(x, "mx_matmul")
     codes, scales = _stored(codes, scales, 2, x.size(-1), dev, "mx_matmul")
     if x.requires_grad and torch.is_grad_enabled():
         _hip.note_stream(x, "mx_matmul")
@@ -194,6 +196,7 @@ def mx_grouped_swiglu(x: Tensor, gate: tuple, up: tuple, down: tuple, offsets: T
         raise ValueError(f"{what}: x is [rows, d], got shape {tuple(x.shape)}")
     if x.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("gradients through quantised experts are not supported")
+    _hip.refuse_tangent(x, what)
     d = x.size(1)
     gate, up = (_stored(*m, 3, d, x.device, f"{what} {n}") for m, n in ((gate, "gate"), (up, "up")))
     experts, ffn = gate[0].shape[:2]

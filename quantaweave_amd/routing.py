@@ -100,11 +100,13 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
     * weight: scores[index], divided by their sum plus 1e-20 where `renormalize`,
       times `scale`.
 
-    Differentiable in logits through weight and scores."""
+    Differentiable in logits through weight and scores; second and
+    forward-mode derivatives are refused."""
     if not logits.is_cuda:
         _hip.require_device(logits, "route_experts")
     if logits.dtype != torch.float32 or logits.dim() < 1:
         raise ValueError(f"route_experts: logits are float32 [..., experts], got {logits.dtype} {tuple(logits.shape)}")
+    _hip.refuse_tangent(logits, "route_experts")
     experts = logits.size(-1)
     top_groups = groups if top_groups is None else top_groups
     check_rule(experts, top_k, score, groups, top_groups, group_score, scale)

@@ -92,6 +92,27 @@ def test_oracle_values_and_quantise_are_inverse():
     assert torch.equal(ref.on_grid(v), v)
 
 
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_tangents_are_refused(monkeypatch, requires_grad):
+    """Before any launch; the device check is passed over, nothing else of the calls."""
+    from torch.autograd import forward_ad
+
+    from quantaweave_amd import _hip
+
+    monkeypatch.setattr(_hip, "require_device", lambda t, what: None)
+    x = torch.randn(4, 64, requires_grad=requires_grad)
+    gen = torch.Generator().manual_seed(0)
+    wide, stack, down = (ref.stored(gen, *s) for s in ((8, 64), (2, 32, 64), (2, 64, 32)))
+    calls = [lambda t: qa.mx_matmul(t, *wide), lambda t: qa.route_experts(t, 2)]
+    if not requires_grad:
+        calls.append(lambda t: qa.mx_grouped_swiglu(t, stack, stack, down, torch.tensor([0, 1, 4]).int()))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.randn(4, 64))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+
+
 def test_backward_under_capture_is_refused_while_a_graph_of_another_stream_lives(monkeypatch):
     """The streams and the capture are stood in for: the refusal is decided on the host, before any launch."""
     from quantaweave_amd import _hip
