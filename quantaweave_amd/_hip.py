@@ -70,16 +70,28 @@ def refuse_tangent(t: torch.Tensor, what: str) -> None:
 _STREAM_KEY = "quantaweave stream"
 
 
-def note_stream(t: torch.Tensor, what: str) -> None:
-    """Called by a differentiable operator before it records a node on `t` (grad
-    mode on, `t` requiring grad).  The node that takes t's gradient is bound to
-    the stream it was first made on and lives as long as any graph through it
-    does.  A backward pass recorded into a HIP graph while it is bound to another
-    stream makes that stream wait inside the capture, which ends the process at
-    the capture's end; so the node is marked with its stream here, and a call
-    under capture that finds another stream's mark is refused."""
+def gradient_node(t: torch.Tensor) -> torch.autograd.graph.Node:
+    """The node that takes t's gradient (grad mode on, `t` requiring grad), marked
+    with the stream it is first seen on.  A leaf holds its node weakly: a
+    differentiable operator keeps the returned one until its own node refers to it,
+    or the mark is gone with it."""
     node = t.view_as(t).grad_fn.next_functions[0][0] if t.grad_fn is None else t.grad_fn
-    here = raw_stream(t.device)
-    if node.metadata.setdefault(_STREAM_KEY, here) != here and torch.cuda.is_current_stream_capturing():
+    node.metadata.setdefault(_STREAM_KEY, raw_stream(t.device))
+    return node
+
+
+def note_stream(t: torch.Tensor | torch.autograd.graph.Node, what: str, device: torch.device | None = None) -> None:
+    """Called by a differentiable operator's backward pass with the node that its
+    gradient goes to (of a tensor on `device`; or with the tensor, whose node is
+    marked then).  That node is bound to the stream it was made on and lives as long
+    as any graph through it does.  A backward pass recorded into a HIP graph while it
+    is bound to another stream makes that stream wait inside the capture, which ends
+    the process at the capture's end; so it is refused here, before the gradient is
+    handed on.  It is known of nodes that these operators met before the capture;
+    those that other operations alone have met carry no mark."""
+    if isinstance(t, torch.Tensor):
+        t, device = gradient_node(t), t.device
+    here = raw_stream(device)
+    if t.metadata.get(_STREAM_KEY, here) != here and torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what}: the input still belongs to a graph made on another stream, so its backward pass "
                            "cannot be captured; drop that graph's results (or detach the input) before the capture")

@@ -110,10 +110,11 @@ def mx_dequantize(codes: Tensor, scales: Tensor, cols: int, dtype: torch.dtype =
     return out
 
 
-def _matmul(flat: Tensor, stride: int, codes: Tensor, scales: Tensor) -> Tensor:
+def _matmul(x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
+    flat, stride = _rows(x, "mx_matmul")
     (rows, k), n = flat.shape, codes.size(0)
     dev = flat.device
-    out = torch.empty((rows, n), dtype=flat.dtype, device=dev)
+    out = torch.empty((*x.shape[:-1], n), dtype=flat.dtype, device=dev)
     if rows and n:
         act, at = _hip.act_code(flat, "mx_matmul"), _hip.ptr(flat)
         nbytes = _lib.load().qw_mx_matmul_workspace_bytes(at, act, stride, rows, n, k)
@@ -129,23 +130,24 @@ class _MxMatmul(torch.autograd.Function):
     The stored matrix is whole numbers and gets none."""
 
     @staticmethod
-    def forward(ctx, flat: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
-        rows, stride = _rows(flat, "mx_matmul")
+    def forward(ctx, x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
         ctx.save_for_backward(codes, scales)
-        ctx.cols, ctx.dtype = flat.size(1), flat.dtype
-        return _matmul(rows, stride, codes, scales)
+        ctx.shape, ctx.dtype = x.shape, x.dtype
+        return _matmul(x, codes, scales)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad: Tensor):
         if not ctx.needs_input_grad[0]:
             return None, None, None
+        _hip.note_stream(ctx.next_functions[0][0], "mx_matmul", grad.device)
         codes, scales = ctx.saved_tensors
         grad = grad.to(ctx.dtype).contiguous()
         if grad.data_ptr() % 16:
             grad = grad.clone()  # the matrix cores' loads
-        rows, n, k = grad.size(0), codes.size(0), ctx.cols
-        gx = torch.empty(rows, k, dtype=ctx.dtype, device=grad.device)
+        gx = torch.empty(ctx.shape, dtype=ctx.dtype, device=grad.device)
+        n, k = codes.size(0), ctx.shape[-1]
+        rows = gx.numel() // k
         if rows and n:
             act = _hip.act_code(grad, "mx_matmul")
             nbytes = _lib.load().qw_mx_matmul_backward_workspace_bytes(rows, n, k, act)
@@ -172,11 +174,9 @@ def mx_matmul(x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
     _hip.refuse_tangent(x, "mx_matmul")
     codes, scales = _stored(codes, scales, 2, x.size(-1), dev, "mx_matmul")
     if x.requires_grad and torch.is_grad_enabled():
-        _hip.note_stream(x, "mx_matmul")
-        out = _MxMatmul.apply(x.reshape(-1, x.size(-1)), codes, scales)
-    else:
-        out = _matmul(*_rows(x, "mx_matmul"), codes, scales)
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], codes.size(0))
+        node = _hip.gradient_node(x)  # held until the result's graph holds it
+        return _MxMatmul.apply(x, codes, scales)
+    return _matmul(x, codes, scales)
 
 
 def mx_grouped_swiglu(x: Tensor, gate: tuple, up: tuple, down: tuple, offsets: Tensor,

@@ -58,7 +58,11 @@ class _RouteExperts(torch.autograd.Function):
     def backward(ctx, _index, d_weight, d_scores):
         scores, index = ctx.saved_tensors
         top_k, score, _bias, _groups, _top_groups, _group_score, renormalize, scale = ctx.rule
-        t, e = scores.shape
+        if not ctx.needs_input_grad[0]:
+            return None, None
+        _hip.note_stream(ctx.next_functions[0][0], "route_experts", scores.device)
+        e = scores.size(-1)
+        t = scores.numel() // e
         out = torch.empty_like(scores)
         if t:
             dw = None if d_weight is None else d_weight.float().contiguous()
@@ -70,12 +74,12 @@ class _RouteExperts(torch.autograd.Function):
 
 def _route(logits: Tensor, top_k: int, score: str, bias: Optional[Tensor], groups: int, top_groups: int,
            group_score: str, renormalize: bool, scale: float) -> tuple[Tensor, Tensor, Tensor]:
-    t, e = logits.shape
-    dev = logits.device
+    dev, lead, e = logits.device, logits.shape[:-1], logits.size(-1)
     logits = logits.contiguous()
+    t = logits.numel() // e
     scores = torch.empty_like(logits)
-    index = torch.empty((t, top_k), dtype=torch.int32, device=dev)
-    weight = torch.empty((t, top_k), dtype=torch.float32, device=dev)
+    index = torch.empty((*lead, top_k), dtype=torch.int32, device=dev)
+    weight = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
     if t:
         _hip.call_on(dev, "qw_moe_route_scored_from_logits", _hip.ptr(logits), t, e, top_k, SCORES[score],
                      _hip.ptr(bias), groups, top_groups, GROUP_SCORES[group_score], int(renormalize), scale,
@@ -114,14 +118,8 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
         if tuple(bias.shape) != (experts,) or bias.device != logits.device:
             raise ValueError(f"route_experts: bias is [{experts}] on {logits.device}")
         bias = bias.detach().float().contiguous()
-    flat = logits if logits.dim() == 2 else logits.reshape(-1, experts)
     rule = (top_k, score, bias, groups, top_groups, group_score, bool(renormalize), float(scale))
     if logits.requires_grad and torch.is_grad_enabled():
-        _hip.note_stream(logits, "route_experts")
-        index, weight, scores = _RouteExperts.apply(flat, rule)
-    else:
-        index, weight, scores = _route(flat.detach(), *rule)
-    if logits.dim() == 2:
-        return index, weight, scores
-    lead = logits.shape[:-1]
-    return index.view(*lead, top_k), weight.view(*lead, top_k), scores.view(*lead, experts)
+        node = _hip.gradient_node(logits)  # held until the result's graph holds it
+        return _RouteExperts.apply(logits, rule)
+    return _route(logits.detach(), *rule)

@@ -413,6 +413,35 @@ def test_backward_captured_and_replayed():
             assert torch.equal(a, b)
 
 
+def test_backward_captured_beside_an_eager_graph_of_its_leaf_is_refused():
+    """And a forward pass captured beside it is not; without the eager graph both are captured."""
+    g = gen(47)
+    w, x = cuda(ref.stored(g, 64, 128)), ref.rows(g, 24, 128, torch.bfloat16).cuda().requires_grad_(True)
+    z = torch.randn(24, 32, generator=g).cuda().requires_grad_(True)
+    for op, leaf in ((lambda: qa.mx_matmul(x, *w), x), (lambda: qa.route_experts(z, 4)[1], z)):
+        kept = op()
+        dy = torch.ones_like(kept)
+        (eager,) = torch.autograd.grad(kept, leaf, dy, retain_graph=True)
+        forward, refused, both = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(forward):
+            alone = op()
+        for _ in range(2):
+            forward.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(alone, kept)
+        del alone
+        with pytest.raises(RuntimeError, match="another stream"):
+            with torch.cuda.graph(refused):
+                torch.autograd.grad(op(), leaf, dy)
+        del kept
+        with torch.cuda.graph(both):
+            (captured,) = torch.autograd.grad(op(), leaf, dy)
+        for _ in range(2):
+            both.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(captured, eager)
+
+
 def test_refusals():
     g = gen(1)
     x = torch.randn(4, 96, generator=g).cuda()

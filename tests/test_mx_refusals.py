@@ -92,6 +92,36 @@ def test_oracle_values_and_quantise_are_inverse():
     assert torch.equal(ref.on_grid(v), v)
 
 
+@pytest.mark.parametrize("lead", [(5,), (2, 3)])
+def test_a_captured_forward_is_taken_and_its_backward_refused_beside_a_graph_of_another_stream(monkeypatch, lead):
+    """Through the operators, with streams, capture, device check and launches stood in for."""
+    from quantaweave_amd import _hip
+
+    now = {"stream": 1, "capturing": False}
+    monkeypatch.setattr(_hip, "stream", lambda device: now["stream"])
+    monkeypatch.setattr(_hip, "call_on", lambda *args: None)
+    monkeypatch.setattr(_hip, "require_device", lambda t, what: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    w = ref.stored(torch.Generator().manual_seed(0), 8, 64)
+    for what, op in (("mx_matmul", lambda t: qa.mx_matmul(t, *w)), ("route_experts", lambda t: qa.route_experts(t, 2)[1])):
+        leaf = torch.randn(*lead, 64, requires_grad=True)
+        now.update(stream=1, capturing=False)
+        kept = op(leaf)  # the eager graph
+        now.update(stream=7, capturing=True)
+        y = op(leaf)     # a forward pass alone is no fault
+        with pytest.raises(RuntimeError, match=f"{what}.*another stream"):
+            torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
+        now.update(capturing=False)
+        assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].shape == leaf.shape  # no capture: torch's own waits do
+        now.update(stream=1, capturing=True)
+        y = op(leaf)
+        torch.autograd.grad(y, leaf, torch.ones_like(y))  # captured on the stream the graph was made on
+        del kept, y
+        now.update(stream=7)
+        y = op(leaf)     # the graph is gone, and its node with it
+        torch.autograd.grad(y, leaf, torch.ones_like(y))
+
+
 @pytest.mark.parametrize("requires_grad", [False, True])
 def test_forward_mode_tangents_are_refused(monkeypatch, requires_grad):
     """Before any launch; the device check is passed over, nothing else of the calls."""
