@@ -353,7 +353,8 @@ int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1,
   a.experts = static_cast<int>(E);
   a.parts = gy1 ? 2 : 1;
   const int64_t nt = ceil_div(K, TR_N);
-  const bool tall = tall_tiles(row_tiles(rows, E, 256) * nt);
+  // (the last row's bytes from a tile's first are 32 bits: 256 rows to N = 2^23, 128 to 2^24)
+  const bool tall = N <= (1 << 22) && tall_tiles(row_tiles(rows, E, 256) * nt);
   const int64_t blocks = kXcds * nt * ceil_div(ceil_div(rows, tall ? 256 : 128) + E, kXcds);
   if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many tiles for one product");
   auto go = [&](auto dt, auto bt, auto cdt) {

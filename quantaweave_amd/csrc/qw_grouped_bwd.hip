@@ -389,10 +389,15 @@ int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dt
 // of 4, gy and w on 16 bytes.
 int grouped_f32_dx(const float* gy, const float* w, int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets,
                    int64_t rows, float* gx, hipStream_t stream) {
-  const dim3 g(static_cast<unsigned>(ceil_div(K, FB_T)), static_cast<unsigned>(ceil_div(rows, FB_T)));
-  grouped_f32_kernel<false><<<g, 256, 0, stream>>>(gy, w, offsets, static_cast<int>(N), static_cast<int>(w_pitch),
-                                                   static_cast<int>(K), static_cast<int>(rows), 0, gx);
-  QW_LAUNCH_CHECK("grouped_f32_kernel");
+  const int64_t most = int64_t{65535} * FB_T;  // rows of one grid; the kernel clamps the offsets to a launch's rows
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t some = rows - r < most ? rows - r : most;
+    const dim3 g(static_cast<unsigned>(ceil_div(K, FB_T)), static_cast<unsigned>(ceil_div(some, FB_T)));
+    grouped_f32_kernel<false><<<g, 256, 0, stream>>>(gy + r * N, w, offsets, static_cast<int>(N),
+                                                     static_cast<int>(w_pitch), static_cast<int>(K),
+                                                     static_cast<int>(some), 0, gx + r * K);
+    QW_LAUNCH_CHECK("grouped_f32_kernel");
+  }
   return QW_OK;
 }
 

@@ -1,5 +1,7 @@
 // C ABI entry points of the microscaled (MX) operators: argument checks,
 // workspace carving and kernel selection.
+#include <algorithm>
+
 #include "qw_mx_product.h"
 
 namespace qw {
@@ -71,7 +73,8 @@ struct RowsGradient {
     const int64_t slice = dtype == QW_F32 ? 4 : 64, load = dtype == QW_F32 ? 4 : 8, size = dtype == QW_F32 ? 4 : 2;
     n = ceil_div(out_features, slice) * slice;
     pitch = ceil_div(in_features, load) * load;
-    copied = dtype == QW_F16 || n != out_features;
+    // (the vector-ALU kernel, which takes a gy off 16 bytes, goes to 65535 * 64 outputs)
+    copied = dtype == QW_F16 || n != out_features || n > 65535 * 64;
     Carver c(workspace);
     offsets = c.take<int32_t>(2);
     w = c.take<char>(static_cast<size_t>(n) * pitch * size);
@@ -194,8 +197,6 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
     return set_error(QW_ERR_WORKSPACE, "mx_matmul_backward needs a workspace of %zu bytes, got %zu", need,
                      workspace_bytes);
   const RowsGradient g(workspace, rows, out_features, in_features, dtype);
-  QW_REQUIRE(ceil_div(rows, 64) <= 65535 && g.n <= 1 << 22, "sizes out of range for a gradient: %lld rows, %lld out_features",
-             (long long)rows, (long long)out_features);
   const hipStream_t s = as_stream(stream);
   mx_offsets_kernel<<<1, 1, 0, s>>>(g.offsets, static_cast<int>(rows));
   QW_LAUNCH_CHECK("mx_offsets_kernel");
@@ -203,8 +204,14 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
   auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   if (!g.copied && !aligned(grad_out)) {  // no copy and no 16-byte loads: the vector-ALU kernel
     st = mx_dequantize(codes, scales, out_features, in_features, g.w, wdt, out_features, s);
-    return st ? st : grouped_matmul_backward(grad_out, nullptr, g.w, dtype, dtype, 1, out_features, in_features,
-                                             g.offsets, rows, rows, grad_x, 0, nullptr, dtype, nullptr, 0, s);
+    const int64_t size = dtype == QW_F32 ? 4 : 2, most = 65535 * 64;  // rows of one grid
+    for (int64_t r = 0; !st && r < rows; r += most) {
+      const int64_t some = std::min(most, rows - r);
+      st = grouped_matmul_backward(static_cast<const char*>(grad_out) + r * out_features * size, nullptr, g.w, dtype,
+                                   dtype, 1, out_features, in_features, g.offsets, some, some,
+                                   static_cast<char*>(grad_x) + r * in_features * size, 0, nullptr, dtype, nullptr, 0, s);
+    }
+    return st;
   }
   st = mx_dequantize(codes, scales, out_features, g.pitch, g.w, wdt, g.n, s);
   if (st) return st;

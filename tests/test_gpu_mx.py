@@ -218,6 +218,41 @@ def test_matmul_gradient_of_any_width(dtype, rows, cols, n):
         assert (out[:start] == 3.0).all() and (out[start + rows * cols:] == 3.0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,n", [(65535 * 64 + 70, 32, 4), (70, 16, (1 << 22) + 72)])
+def test_matmul_gradient_of_what_the_product_takes(dtype, rows, cols, n):
+    """More rows, and more outputs, than one grid or one tile's 32-bit offsets hold."""
+    g = torch.Generator("cuda").manual_seed(rows % 1000)
+    codes = torch.randint(0, 256, (n, 64), dtype=torch.uint8, device="cuda", generator=g)
+    codes[:, cols // 2:] = 0
+    scales = torch.randint(118, 122, (n, 4), dtype=torch.uint8, device="cuda", generator=g)
+    x = torch.randn(rows, cols, device="cuda", generator=g).to(dtype).requires_grad_(True)
+    y = qa.mx_matmul(x, codes, scales)
+    dy = torch.randn(rows, n, device="cuda", generator=g).to(dtype)
+    (gx,) = torch.autograd.grad(y, x, dy)
+    act, lib = _hip.act_code(dy, "test"), _lib.load()
+    nbytes = lib.qw_mx_matmul_backward_workspace_bytes(rows, n, cols, act)
+    ws, out = torch.empty(nbytes, dtype=torch.uint8, device="cuda"), torch.empty_like(gx)
+    off = torch.empty(rows * n + 1, dtype=dtype, device="cuda")[1:].view(rows, n).copy_(dy)  # off 16 bytes
+    _lib.call("qw_mx_matmul_backward", _hip.ptr(off), act, rows, _hip.ptr(codes), _hip.ptr(scales), n, cols,
+              _hip.ptr(out), _hip.ptr(ws), nbytes, _hip.stream(out.device))
+    for r in sorted({0, max(rows - 500, 0)}):  # the first rows and the last
+        d = dy[r:r + 500]
+        want = torch.zeros(d.size(0), cols, dtype=torch.float64, device="cuda")
+        total = torch.zeros_like(want)
+        for at in range(0, n, 1 << 18):
+            wv = qa.mx_dequantize(codes[at:at + (1 << 18)], scales[at:at + (1 << 18)], cols).double()
+            part = d[:, at:at + (1 << 18)].double()
+            want += part @ wv
+            total += part.abs() @ wv.abs()
+        # n terms (2 n of fp16's parts, n products rounded of fp32), each addition off by 2^-24 of the sum's magnitudes
+        err = (2 * n + 8) * (1 + 2.0 ** -7) * ref.EPS24 * total
+        # where n is past 2^20 that is no bound; the additions' errors are as good as independent: sixteen deviations
+        err = torch.minimum(err, 16 * (2 * n) ** 0.5 * ref.EPS24 * total)
+        for got in (gx, out):
+            close(got[r:r + 500], want.cpu(), ref.allowed(want, err, dtype).cpu())
+
+
 @pytest.mark.parametrize("rows,cols,n", [(1, 33, 7), (5, 96, 64), (70, 264, 130), (300, 512, 200)])
 @pytest.mark.parametrize("low,high", [(87, 158), (90, 91), (100, 101), (141, 142), (150, 151), (60, 230)])
 def test_fp16_gradient_over_the_range_of_the_scales(rows, cols, n, low, high):
