@@ -67,10 +67,16 @@ __device__ __forceinline__ s16x4 tr_read(const lds_s16x4* __restrict__ at) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>(at));
 }
 
-// CDT: the result's type (DT, QW_F32, or QW_F16 of bf16 operands)
+// CDT: the result's type (DT, QW_F32, or QW_F16 of bf16 operands: the rows are then
+// sums of two, a0 + a1.  Both halves of a row tile are in LDS, sub-tiles 2 p of a
+// wave from a0 and 2 p + 1, the same rows, from a1; B is read once for both and the
+// pair's accumulators are added at the end).
 template <int DT, int SM, bool RED, bool BT, int CDT>
 __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
+  constexpr bool SPLIT = CDT == QW_F16 && DT == QW_BF16;
   constexpr int TM = 32 * SM, NP = SM / 2, NT = 4;
+  constexpr int ROWS = SPLIT ? TM / 2 : TM;  // rows of the result
+  static_assert(!SPLIT || !RED, "sums of two rows are of mode rows");
   constexpr int A_STAGE = TM * TR_K * 2, B_STAGE = TR_N * TR_K * 2;
   constexpr int AL = A_STAGE / 1024 / TR_WAVES, BL = B_STAGE / 1024 / TR_WAVES;
   constexpr int ST = tr_stages<SM>(), AHEAD = ST - 1;
@@ -91,12 +97,12 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
   if constexpr (!RED) {
     int local = 0;
     nt = j % n_nt;
-    e = find_tile(p.offsets, p.experts, p.rows, TM, (j / n_nt) * kXcds + xcd, &local);
+    e = find_tile(p.offsets, p.experts, p.rows, ROWS, (j / n_nt) * kXcds + xcd, &local);
     if (e < 0) return;
     const int lo = min(max(p.offsets[e], 0), p.rows), hi = min(p.offsets[e + 1], p.rows);
-    row0 = lo + local * TM;
+    row0 = lo + local * ROWS;
     m0 = 0;
-    mcount = min(TM, hi - static_cast<int>(row0));
+    mcount = min(ROWS, hi - static_cast<int>(row0));
     if (mcount <= 0) return;
     len = p.k;
     KT = p.parts * (p.k / TR_K);
@@ -126,7 +132,8 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
     if constexpr (RED)
       a_off[q] = 2u * (static_cast<uint32_t>(r) * p.lda + min(m0 + 8 * (piece ^ (tr_swz(r) << 1)), p.m - 8));
     else
-      a_off[q] = 2u * (static_cast<uint32_t>(min(r, mcount - 1)) * p.lda + 8 * (piece ^ ((r >> 1) & 7)));
+      a_off[q] = 2u * (static_cast<uint32_t>(min(SPLIT ? r / 64 * 32 + r % 32 : r, mcount - 1)) * p.lda +
+                       8 * (piece ^ ((r >> 1) & 7)));
   }
 #pragma unroll
   for (int q = 0; q < BL; ++q) {
@@ -169,9 +176,11 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
       }
     } else {
 #pragma unroll
-      for (int q = 0; q < AL; ++q)
-        __builtin_amdgcn_global_load_lds(static_cast<const void*>(as + a_off[q]),
-                                         (lds_void*)(sa + (wave + q * TR_WAVES) * 1024), 16, 0, 0);
+      for (int q = 0; q < AL; ++q) {
+        const int g = wave + q * TR_WAVES;
+        const char* const from = SPLIT && g / 4 % 2 ? a_second + ks * a_step : as;  // 32 rows of LDS in turn
+        __builtin_amdgcn_global_load_lds(static_cast<const void*>(from + a_off[q]), (lds_void*)(sa + g * 1024), 16, 0, 0);
+      }
 #pragma unroll
       for (int q = 0; q < BL; ++q)
         __builtin_amdgcn_global_load_lds(static_cast<const void*>(bs + b_off[q]),
@@ -255,7 +264,8 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
   };
   // pairs of sub-tiles wholly past the tile's rows are not multiplied
   const int active = (mcount + 15) / 16;
-  const int npa = __builtin_amdgcn_readfirstlane(((active > wm ? (active - wm + 1) / 2 : 0) + 1) / 2);
+  const int mine = active > wm ? (active - wm + 1) / 2 : 0;  // this wave's sub-tiles of rows
+  const int npa = __builtin_amdgcn_readfirstlane(SPLIT ? mine : (mine + 1) / 2);
   if (npa >= NP) k_loop(std::integral_constant<int, NP>{});
   else if (NP == 4 && npa == 3) k_loop(std::integral_constant<int, NP == 4 ? 3 : 1>{});
   else if (NP == 4 && npa == 2) k_loop(std::integral_constant<int, NP == 4 ? 2 : 1>{});
@@ -267,7 +277,7 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
   // four columns go as one store where every row of the result starts on as many
   const bool fours = CDT == QW_F32 || (p.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(c) % 8 == 0);
 #pragma unroll
-  for (int i = 0; i < SM; ++i) {
+  for (int i = 0; i < (SPLIT ? NP : SM); ++i) {
     const int m = (wm + 2 * i) * 16 + l16;
     if (m >= mcount) continue;
     const int64_t row = (c_row0 + m) * p.ldc + n0;
@@ -275,7 +285,8 @@ __global__ __launch_bounds__(TR_THREADS) void gemm_tr_kernel(const TrArgs p) {
     for (int t = 0; t < NT; ++t) {
       const int n = wn * 64 + 16 * t + 4 * lq;
       if (n0 + n >= p.n) continue;
-      const f32x4 v = acc[i][t];
+      f32x4 v = acc[SPLIT ? 2 * i : i][t];
+      if constexpr (SPLIT) v += acc[2 * i + 1][t];
       if constexpr (CDT == QW_F32) {
         *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(c) + row + n) = v;
       } else if (fours) {
@@ -333,9 +344,9 @@ bool gemm_tr_dx_fits(const void* gy, const void* w, const void* gx, int64_t E, i
 }
 
 // w_pitch: elements of a row of w, K or more, a multiple of 8; with it K may be any
-// and gx start anywhere.  gx_dtype: dtype, or QW_F16 with plain bf16 operands.
+// and gx start anywhere.
 int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1, int dtype, bool tiled, int64_t E,
-               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx, int gx_dtype,
+               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx,
                hipStream_t stream) {
   TrArgs a{};
   a.a0 = static_cast<const uint16_t*>(gy0);
@@ -357,16 +368,38 @@ int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1,
   const bool tall = N <= (1 << 22) && tall_tiles(row_tiles(rows, E, 256) * nt);
   const int64_t blocks = kXcds * nt * ceil_div(ceil_div(rows, tall ? 256 : 128) + E, kXcds);
   if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many tiles for one product");
-  auto go = [&](auto dt, auto bt, auto cdt) {
-    constexpr int DT = decltype(dt)::value, CDT = decltype(cdt)::value;
-    return tall ? launch_tr<DT, 8, false, decltype(bt)::value, CDT>(a, blocks, stream)
-                : launch_tr<DT, 4, false, decltype(bt)::value, CDT>(a, blocks, stream);
+  auto go = [&](auto dt, auto bt) {
+    constexpr int DT = decltype(dt)::value;
+    return tall ? launch_tr<DT, 8, false, decltype(bt)::value, DT>(a, blocks, stream)
+                : launch_tr<DT, 4, false, decltype(bt)::value, DT>(a, blocks, stream);
   };
   using H = std::integral_constant<int, QW_F16>;
   using B = std::integral_constant<int, QW_BF16>;
-  if (gx_dtype != dtype) return go(B{}, std::false_type{}, H{});
-  if (dtype == QW_F16) return tiled ? go(H{}, std::true_type{}, H{}) : go(H{}, std::false_type{}, H{});
-  return tiled ? go(B{}, std::true_type{}, B{}) : go(B{}, std::false_type{}, B{});
+  if (dtype == QW_F16) return tiled ? go(H{}, std::true_type{}) : go(H{}, std::false_type{});
+  return tiled ? go(B{}, std::true_type{}) : go(B{}, std::false_type{});
+}
+
+// gx (fp16) = (high + low) . w of one group, bf16 operands; w_pitch, K and gx as above.
+int gemm_tr_dx_split(const void* high, const void* low, const void* w, int64_t N, int64_t K, int64_t w_pitch,
+                     const int32_t* offsets, int64_t rows, void* gx, hipStream_t stream) {
+  TrArgs a{};
+  a.a0 = static_cast<const uint16_t*>(high);
+  a.a1 = static_cast<const uint16_t*>(low);
+  a.b0 = a.b1 = static_cast<const uint16_t*>(w);
+  a.c0 = a.c1 = gx;
+  a.offsets = offsets;
+  a.lda = static_cast<int>(N);
+  a.ldb = static_cast<int>(w_pitch);
+  a.ldc = a.n = static_cast<int>(K);
+  a.rows = static_cast<int>(rows);
+  a.k = static_cast<int>(N);
+  a.experts = a.parts = 1;
+  const int64_t nt = ceil_div(K, TR_N);
+  const bool tall = tall_tiles(row_tiles(rows, 1, 128) * nt);
+  const int64_t blocks = kXcds * nt * ceil_div(ceil_div(rows, tall ? 128 : 64) + 1, kXcds);
+  if (blocks > INT32_MAX) return set_error(QW_ERR_UNSUPPORTED, "too many tiles for one product");
+  return tall ? launch_tr<QW_BF16, 8, false, false, QW_F16>(a, blocks, stream)
+              : launch_tr<QW_BF16, 4, false, false, QW_F16>(a, blocks, stream);
 }
 
 // dW of one product, or of two with the same x (gy1, gw1 non-null).

@@ -288,7 +288,7 @@ int gemm_grouped_backward(const void* gy, const void* x, const void* w, int dtyp
 bool gemm_tr_dx_fits(const void* gy, const void* w, const void* gx, int64_t E, int64_t N, int64_t K, int64_t rows,
                      bool pair, bool tiles128);
 int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1, int dtype, bool tiled, int64_t E,
-               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx, int gx_dtype,
+               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx,
                hipStream_t stream);
 bool gemm_tr_dw_fits(const void* gy, const void* x, const void* gw, int64_t E, int64_t N, int64_t K);
 int gemm_tr_dw(const void* gy0, const void* gy1, const void* x, int dtype, int64_t E, int64_t N, int64_t K,
@@ -325,7 +325,7 @@ int grouped_matmul_backward(const void* gy, const void* x, const void* w, int dt
   // 256-column tiles over the operands as they lie (no workspace used)
   if (is_half(dtype) && gx != nullptr && !accumulate && rows > 0 &&
       gemm_tr_dx_fits(gy, w, gx, E, N, K, rows, false, core_dx)) {
-    const int st = gemm_tr_dx(gy, nullptr, w, nullptr, dtype, tiled, E, N, K, K, offsets, rows, gx, dtype, stream);
+    const int st = gemm_tr_dx(gy, nullptr, w, nullptr, dtype, tiled, E, N, K, K, offsets, rows, gx, stream);
     if (st) return st;
     gx = nullptr;
   }
@@ -415,7 +415,7 @@ int grouped_matmul_backward_pair(const void* gy_a, const void* gy_b, const void*
   // one accumulator for both: one rounding instead of two, and grad_x written once
   if (is_half(dtype) && gx != nullptr && rows > 0 && gemm_tr_dx_fits(gy_a, w_a, gx, E, N, K, rows, true, false) &&
       gemm_tr_dx_fits(gy_b, w_b, gx, E, N, K, rows, true, false)) {
-    st = gemm_tr_dx(gy_a, gy_b, w_a, w_b, dtype, wfmt != dtype, E, N, K, K, offsets, rows, gx, dtype, stream);
+    st = gemm_tr_dx(gy_a, gy_b, w_a, w_b, dtype, wfmt != dtype, E, N, K, K, offsets, rows, gx, stream);
     if (st) return st;
     gx = nullptr;
   }

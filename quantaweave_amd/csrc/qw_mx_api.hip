@@ -16,8 +16,10 @@ int gemm_dx(const void* gy, const void* w, int64_t N, int64_t K, int64_t w_pitch
 bool gemm_tr_dx_fits(const void* gy, const void* w, const void* gx, int64_t E, int64_t N, int64_t K, int64_t rows,
                      bool pair, bool tiles128);
 int gemm_tr_dx(const void* gy0, const void* gy1, const void* w0, const void* w1, int dtype, bool tiled, int64_t E,
-               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx, int gx_dtype,
+               int64_t N, int64_t K, int64_t w_pitch, const int32_t* offsets, int64_t rows, void* gx,
                hipStream_t stream);
+int gemm_tr_dx_split(const void* high, const void* low, const void* w, int64_t N, int64_t K, int64_t w_pitch,
+                     const int32_t* offsets, int64_t rows, void* gx, hipStream_t stream);
 
 namespace {
 
@@ -57,10 +59,10 @@ MxMatrix matrix(const void* codes, const void* scales) {
 //
 // The matrix is held in bf16 for 16-bit rows, fp16 ones too: stored weights reach
 // from 2^-128 to 6 * 2^127, past fp16 at both ends, and bf16 has their range and more
-// bits than a code.  fp16's eleven bits of gy then go as two bf16 numbers, whose
-// products with W are summed in one fp32 accumulator.  (The matrix in fp16 took half
-// the instructions, 110 us instead of 210 for 1024 rows, 1024 columns and 7168 outputs,
-// and was right for scales of 2^-23 to 2^13 alone.)
+// bits than a code.  fp16's eleven bits of gy then go as two bf16 numbers whose fp32
+// sums are added before the one rounding.  (The matrix in fp16 took half the
+// instructions and was right for scales of 2^-23 to 2^13 alone: 1024 rows, 1024
+// columns and 7168 outputs 110 us a call, 118 so; 8000 rows of 64 columns 104 and 161.)
 struct RowsGradient {
   int64_t n, pitch;  // W's padded rows and columns
   bool copied;       // gy is taken from `rows`
@@ -222,12 +224,13 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
   if (dtype == QW_F32)
     return grouped_f32_dx(static_cast<const float*>(gy), static_cast<const float*>(g.w), g.n, in_features, g.pitch,
                           g.offsets, rows, static_cast<float*>(grad_x), s);
+  if (dtype == QW_F16)
+    return gemm_tr_dx_split(gy, g.low, g.w, g.n, in_features, g.pitch, g.offsets, rows, grad_x, s);
   // tiles of 128 x 128 as in the grouped backward, which need whole fours and 16-byte rows of results
-  const bool tiles128 = dtype == QW_BF16 && in_features % 4 == 0 && aligned(grad_x);
+  const bool tiles128 = in_features % 4 == 0 && aligned(grad_x);
   if (tiles128 && !gemm_tr_dx_fits(gy, g.w, grad_x, 1, g.n, in_features, rows, false, true))
     return gemm_dx(gy, g.w, g.n, in_features, g.pitch, g.offsets, rows, grad_x, s);
-  return gemm_tr_dx(gy, dtype == QW_F16 ? g.low : nullptr, g.w, dtype == QW_F16 ? g.w : nullptr, QW_BF16, false, 1, g.n,
-                    in_features, g.pitch, g.offsets, rows, grad_x, dtype, s);
+  return gemm_tr_dx(gy, nullptr, g.w, nullptr, QW_BF16, false, 1, g.n, in_features, g.pitch, g.offsets, rows, grad_x, s);
 }
 
 size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t d_model, int64_t d_ff) {
