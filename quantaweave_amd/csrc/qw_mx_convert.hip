@@ -111,21 +111,23 @@ __global__ __launch_bounds__(kConvertThreads) void mx_prepare_kernel(const void*
 
 // A lane turns four bytes of codes into eight numbers: code times scale is exact
 // in fp32 (subnormals included) and is rounded once to the output type.  Rows of
-// `cols` columns are written, which may reach into the stored padding; pieces from
-// `stored` on are rows past the stored ones, written as zeros.  Bound by HBM
-// (8192 x 2048 to bf16, 42 MB: 9.1 us, 4.7 TB/s).
-template <int DT>
+// `cols` columns are written, which may reach into the stored padding; with MORE the
+// pieces from `stored` on are rows past the stored ones, written as zeros (a kernel of
+// its own: the comparison took 0.8 us more of every call).  Bound by HBM (8192 x 2048
+// to bf16, 42 MB: 9.0 us, 4.7 TB/s).
+template <int DT, bool MORE>
 __global__ __launch_bounds__(kConvertThreads) void mx_dequantize_kernel(const uint32_t* __restrict__ codes,
                                                                         const uint8_t* __restrict__ scales, int cols,
-                                                                        uint32_t pieces, int64_t stored, int64_t total,
-                                                                        bool aligned, void* __restrict__ out) {
+                                                                        uint32_t pieces, int64_t total, bool aligned,
+                                                                        void* __restrict__ out, int64_t stored) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvertThreads + threadIdx.x;
   if (i >= total) return;
   const int64_t row = total <= INT32_MAX ? static_cast<uint32_t>(i) / pieces : i / pieces;
   const int col = static_cast<int>(i - row * pieces) * 8;
   if (col >= cols) return;
-  const float s = i < stored ? mx_scale_value(scales[i / 4]) : 0.0f;
-  const uint32_t c = i < stored ? codes[i] : 0u;
+  const bool there = !MORE || i < stored;
+  const float s = there ? mx_scale_value(scales[i / 4]) : 0.0f;
+  const uint32_t c = there ? codes[i] : 0u;
   typedef float f32x2_t __attribute__((ext_vector_type(2)));
   const f32x2_t p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0),
                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1),
@@ -276,12 +278,11 @@ int mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t c
   const uint32_t p = static_cast<uint32_t>(pieces);
   const uint32_t* q = static_cast<const uint32_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
-  if (dtype == QW_F32)
-    mx_dequantize_kernel<QW_F32><<<g, kConvertThreads, 0, stream>>>(q, s, c, p, stored, total, aligned, out);
-  else if (dtype == QW_F16)
-    mx_dequantize_kernel<QW_F16><<<g, kConvertThreads, 0, stream>>>(q, s, c, p, stored, total, aligned, out);
-  else
-    mx_dequantize_kernel<QW_BF16><<<g, kConvertThreads, 0, stream>>>(q, s, c, p, stored, total, aligned, out);
+  auto go = [&](auto kernel) { kernel<<<g, kConvertThreads, 0, stream>>>(q, s, c, p, total, aligned, out, stored); };
+  const bool more = out_rows > rows;
+  if (dtype == QW_F32) more ? go(mx_dequantize_kernel<QW_F32, true>) : go(mx_dequantize_kernel<QW_F32, false>);
+  else if (dtype == QW_F16) go(mx_dequantize_kernel<QW_F16, false>);  // (the gradient holds the matrix in bf16)
+  else more ? go(mx_dequantize_kernel<QW_BF16, true>) : go(mx_dequantize_kernel<QW_BF16, false>);
   QW_LAUNCH_CHECK("mx_dequantize_kernel");
   return QW_OK;
 }
