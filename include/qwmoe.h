@@ -536,11 +536,12 @@ int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const v
 
 /* The SwiGLU experts of qw_moe_experts on microscaled weights and rows:
  *   h = silu(gate_e(x_s)) * up_e(x_s),  y[s] = down_e(h)
- * for s in [kept_offsets[e], kept_offsets[e+1]), x_s = x[s] (max_rows rows).  x and h are quantised as by qw_mx_quantize (h from
- * the fp32 sums), products are summed in fp32, y is rounded once to act_dtype.
+ * for s in [kept_offsets[e], kept_offsets[e+1]), x_s = x[s] (max_rows rows).  x and h
+ * are quantised as by qw_mx_quantize (h from the fp32 sums), products are summed in
+ * fp32, y is rounded once to act_dtype.
  * gate, up: stacks [experts, d_ff, d_model]; down: [experts, d_model, d_ff].
  * max_rows bounds kept_offsets[experts]; max_rows_per_expert (0: unknown) only
- * chooses the kernel.  Rows of y past kept_offsets[experts] are left as they were,
+ * chooses the height of the tiles.  Rows of y past kept_offsets[experts] are left as they were,
  * or become zeros where zero_rest != 0. */
 size_t qw_mx_experts_workspace_bytes(int64_t max_rows, int64_t experts, int64_t d_model, int64_t d_ff);
 int qw_mx_experts(const void* x, int act_dtype, int64_t x_row_stride, const int32_t* kept_offsets, int64_t experts,

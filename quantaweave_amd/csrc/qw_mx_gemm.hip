@@ -11,9 +11,9 @@
 // way, so that neither a start nor an epilogue leaves the memory idle.  One tile
 // per workgroup, whose slices of 256 columns began anew with each, took for 16384
 // rows of 64 experts (d 2048, f 1024) 65 us for gate and up and 51 us for down, now
-// 65 and 42; for 4099 rows of popular experts (d 4096, f 1408) 149 and 95 us, now
-// 137 and 75; a product of few tiles has nothing to run on into and loses (1023 x
-// 1408 x 4096: 11.3 us, now 14.1).  Bound by the matrix instructions: 8192 x 2048 x
+// 66 and 42; for 4099 rows of popular experts (d 4096, f 1408) 149 and 95 us, now
+// 139 and 76; a product of few tiles has nothing to run on into and loses (1023 x
+// 1408 x 4096: 11.3 us, now 13.9).  Bound by the matrix instructions: 8192 x 2048 x
 // 7168 in 80 us, 3.0 PFLOP/s; a slice of 320 rows takes about 2000 cycles of which
 // its instructions issue in 1280.
 // Every wave issues the same number of loads per slice (rows past the end are

@@ -51,9 +51,11 @@ int mx_group_chunk(int64_t rows, int64_t groups, int64_t cap);
 // Most chunks that `rows` rows in `groups` groups make, and the bytes of their table.
 inline int64_t mx_max_chunks(int64_t rows, int64_t groups, int chunk) { return ceil_div(rows, chunk) + groups; }
 
-// Whether a product of `rows` rows in `groups` groups is one of few rows: as many as
-// the matrix instruction holds, so that launch_mx_rows reads a weight once (more are
-// another pass over the weights there; the tile kernel's smallest tile is 64 rows).
+// Whether a product of `rows` rows in `groups` groups is one of few rows: on average as
+// many as the matrix instruction holds, so that launch_mx_rows reads a weight once
+// where the groups are even (a group's further sixteens of rows are further passes over
+// its weights there; the tile kernel's smallest tile is 64 rows).  Neither the bound nor
+// the effect of uneven groups was timed with both kernels.
 inline bool mx_few_rows(int64_t rows, int64_t groups) { return rows <= groups * 16; }
 
 // What launch_mx_gemm's rows need beside quantisation, in the same pass.

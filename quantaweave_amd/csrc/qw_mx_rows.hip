@@ -1,5 +1,8 @@
 // Microscaled products of few rows (decoding): each weight is read once per
-// sixteen rows of its group, straight from memory into the matrix instruction.
+// sixteen rows of its group, straight from memory into the matrix instruction.  (A
+// group of many rows beside empty ones is so many passes over its weights: 1024 rows
+// of 64 experts, d 2048, f 1024, evenly 118 us for the experts' products, all rows in
+// one 347 us.)
 //
 // One workgroup owns sixteen rows of a group and 32 columns of the result (two
 // matrices: 32 gate and the matching 32 up columns, one block of the hidden row).
@@ -11,7 +14,7 @@
 // are added in wave order (the same sum whatever the rows beside it).
 //
 // Bound by the weight stream where many experts are touched: 128 rows of 64 experts,
-// d 2048, f 1024, gate and up 45 us (2.7 TB/s), down 19 us (3.3 TB/s).  Bound by
+// d 2048, f 1024, gate and up 43 us (2.9 TB/s), down 20.6 us (3.0 TB/s).  Bound by
 // latency for a single matrix (1 row, 2048 x 7168: 5.6 us, 1.4 TB/s).
 #include "qw_mx_product.h"
 
@@ -22,10 +25,10 @@ namespace {
 constexpr int kRowsM = 16, kRowsN = 32;
 constexpr int kStored = -1;  // XDT of rows that are stored microscaled
 // Steps of 128 columns that a wave takes together.  Two make its two loads of a
-// weight row one 128-byte line (the down product above with one: 24.5 us); two
-// matrices and the numbers of a row leave the registers of two workgroups per unit
-// only one (gate and up above with two, and the next two requested ahead, spilled
-// eighteen registers: 58 us).
+// weight row one 128-byte line (the down product above, in an earlier form, with one
+// 24.5 us and with two 19.2); two matrices and the numbers of a row leave the registers
+// of two workgroups per unit only one (gate and up above with two, and the next two
+// requested ahead, spilled eighteen registers: 58 us).
 template <int XDT, bool GATEUP>
 constexpr int kRowsSteps = GATEUP && XDT != kStored ? 1 : 2;
 // Workgroups that share a group's row chunks: the grid is fixed before the groups'

@@ -61,7 +61,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // step of the maximum; the lower halves are looked at in the rounds where two
 // experts share the largest upper half.
 // Bound by one wave's chain of steps, not by bytes: 1 token of 256 experts in 8
-// groups, k 8: 7.3 us; 8192 tokens: 25.1 us (17 MB, 0.7 TB/s).
+// groups, k 8: 7.4 us; 8192 tokens: 24.3 us (17 MB, 0.7 TB/s).
 template <int EPL>
 __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_kernel(
     const float* __restrict__ logits, int T, int E, int K, const float* __restrict__ bias, ScoredRule rule,
@@ -215,8 +215,9 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_kernel(
 //   dp_j  = scale * (g_j - sum_i g_i s_idx_i / S) / S   (S the renormalising sum; scale * g_j without)
 //   ds_e  = grad_scores_e + sum_{idx_j = e} dp_j
 //   dl_e  = softmax: s_e (ds_e - sum ds s);  sigmoid: ds_e s_e (1 - s_e)
-// An index outside [0, E) is skipped.  8192 tokens of 256 experts, k 8: 10.5 us (17 MB,
-// 1.6 TB/s; the choices are dealt to their lanes one after another).
+// An index outside [0, E) is skipped.  8192 tokens of 256 experts, k 8, with the
+// gradients of both weights and scores: 9.8 us (25 MB, 2.6 TB/s; the choices are dealt
+// to their lanes one after another).
 template <int EPL>
 __global__ __launch_bounds__(kRouteWaves* kWave) void route_scored_backward_kernel(
     const float* __restrict__ scores, const int32_t* __restrict__ top_idx, const float* __restrict__ grad_top_w,

@@ -186,7 +186,8 @@ def mx_grouped_swiglu(x: Tensor, gate: tuple, up: tuple, down: tuple, offsets: T
     x [rows, d]; gate and up (codes, scales) stacks [experts, ffn, d], down
     [experts, d, ffn]; offsets int32 [experts + 1] on x's device, ascending from
     0 (rows past the last offset give zeros); max_rows bounds an expert's rows
-    (None: unknown) and only chooses the kernel.  x and the hidden rows
+    (None: unknown) and only chooses the height of the tiles that more than
+    sixteen rows an expert on average go to.  x and the hidden rows
     silu(gate) * up are quantised on the way, sums are fp32, the result is
     rounded once to x's type.  Not differentiable."""
     what = "mx_grouped_swiglu"

@@ -95,7 +95,8 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
     Returns (index int32 [..., top_k], weight [..., top_k], scores [..., experts]):
 
     * scores: softmax(logits), or sigmoid(logits) per expert;
-    * the choice goes by scores + bias (bias [experts], no gradient): of the
+    * the choice goes by scores + bias (bias [experts], taken in float32, no
+      gradient): of the
       `groups` equal runs of experts the `top_groups` with the highest value
       stay (`group_score`: the sum of the run's two highest, or its highest),
       and of their experts the top_k highest are taken, in descending order.
