@@ -528,7 +528,8 @@ int qw_mx_matmul(const void* x, int act_dtype, int64_t x_row_stride, int64_t row
 /* grad_x [rows, in_features] = grad_out [rows, out_features] @ W, the stored
  * matrix exact but for entries of 2^128 and more (scale bytes 253 and 254), which
  * are infinite, products summed in fp32 and rounded once: the gradient of
- * qw_mx_matmul with the quantisation of x passed over. */
+ * qw_mx_matmul with the quantisation of x passed over.  fp32 and bf16 rows that do
+ * not start on 16 bytes run on a slower kernel where no padded copy is made. */
 size_t qw_mx_matmul_backward_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features, int dtype);
 int qw_mx_matmul_backward(const void* grad_out, int dtype, int64_t rows, const void* codes, const void* scales,
                           int64_t out_features, int64_t in_features, void* grad_x, void* workspace,
